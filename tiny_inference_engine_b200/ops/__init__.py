@@ -1954,3 +1954,8 @@ def attention_decode_kept(q, k_cache, v_cache, out, query_start, context_lens, b
          context_lens.data_ptr(), block_tables.data_ptr(), block_tables.shape[1], q_heads, kv_heads, head_dim, k_cache.shape[2],
          k_cache.shape[0], int(window), int(keep_first), float(scale), float(softcap), _sink_ptr(sink, q_heads), 0, first, n_list, split_keys,
          max_splits, scratch.data_ptr(), counters.data_ptr(), 1 if cluster else 0, _stream())
+
+
+from .kv4 import (Kv4Cache, Kv4Workspace, StepArrays, TABLES_BAD_REQUEST, TABLES_NO_PAGES, TABLES_ROWS, TABLES_SHORT,  # noqa: E402, F401
+                  attention_kv4_decode, attention_kv4_prompt, kv4_append, kv4_cache, kv4_read, kv4_workspace, release_tables, step_arrays,
+                  step_tables)

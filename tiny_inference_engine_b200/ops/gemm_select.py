@@ -316,6 +316,11 @@ def check_status() -> None:
                  12: "an attention kernel waiting for keys and values"}.get(code, f"code {code}")
         if code == 13:
             raise TieError("decode attention was given fewer splits than a context needs; that sequence's output was not written")
+        if code == 15:
+            raise TieError("attention over a cache in 4 bits: a block table is too short for its context or names a page outside of the cache; "
+                           "that sequence's output is invalid")
+        if code == 16:
+            raise TieError("a cache in 4 bits: a slot outside of the cache; nothing was written or read for it")
         raise TieError(f"a kernel gave up after its wait limit ({where}); its output is invalid")
 
 

@@ -117,6 +117,11 @@ _SIGNATURES = {
     "tie_attention_kept_split": [I, P, L, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, F, F, P, P, I, I, I, P, P],
     "tie_attention_prompt_kept": [P, L, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, F, F, P, P],
     "tie_attention_decode_kept": [P, L, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, F, P, P, I, I, I, I, P, P, I, P],
+    "tie_kv4_append": [I, P, P, L, L, P, P, P, P, P, I, I, I, I, L, P],
+    "tie_kv4_read": [I, P, P, P, P, P, P, P, L, L, I, I, I, I, L, P],
+    "tie_attention_kv4": [I, P, L, L, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, L, I, F, P, I, I, P, P, P],
+    "tie_step_tables": [P] * 14 + [I] * 8 + [P],
+    "tie_release_tables": [P] * 6 + [I] * 5 + [P],
     "tie_attention_mixed": [I, P, L, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, F, I, P, I, I, I, P, P],
 }
 
@@ -163,6 +168,8 @@ def library() -> ctypes.CDLL:
         lib.tie_delta_chunk_takes.argtypes = [I, I, I, I, I, I, L, L, P, P, P, P, P, P, P]
         lib.tie_delta_chunk_scratch.restype = c_longlong
         lib.tie_delta_chunk_scratch.argtypes = [I, I, I, I, I]
+        lib.tie_attention_kv4_ctas.restype = c_int
+        lib.tie_attention_kv4_ctas.argtypes = []
         lib.tie_moe_max_tiles.restype = c_int
         lib.tie_moe_max_tiles.argtypes = [c_int, c_int, c_int]
         lib.tie_replay_launcher_id.restype = c_int
