@@ -28,15 +28,24 @@
 // gave up a wait too, and the CTAs of a cluster leave ahead of them together or not at all.)
 // grid = (kv heads, row tiles, sequences x splits): CTAs start in that order with the last row tiles first, so the
 // tiles with the most keys of every kv head run first.
+//
+// KV4: the same over a cache in 4 bits (kv4.cuh), heads of up to 64 or 128 (a multiple of 8; what is missing is zeros) and pages of any size.
+// Four warps take the place of the TMA producer: they read codes and words a tile ahead, take them apart and write the
+// tile as TMA would have. Eight dimensions lie in it in the order 0 4 1 5 2 6 3 7, in which a word of codes comes apart; Q is put into tensor
+// memory in the same order and the outputs are taken out of it again. Keys and values are exact in bfloat16, times 2^-64 (kv4.cuh).
 #include "attention_mma.cuh"
+#include "kv4.cuh"
 #include "umma.cuh"
 #include "launchers.h"
 
 namespace tie {
 
-constexpr int kUmmaAttnThreads = 320;
+constexpr int kUmmaAttnThreads = 320, kUmmaKv4Threads = 384;
 constexpr int kUmmaMaxSplits = 4;
 constexpr int kUmmaSplitKeys = 2049;
+
+// Where dimension d of eight lies in a tile of a cache in 4 bits (KV4 below).
+__host__ __device__ constexpr int ordered(int d) { return (d & ~7) | ((d & 3) << 1) | ((d >> 2) & 1); }
 
 struct UmmaPromptArgs {
   const __nv_bfloat16* q;
@@ -50,10 +59,111 @@ struct UmmaPromptArgs {
   float scale_log2;
   int splits;     // CTAs of a cluster that share out the keys of 256 rows (1: no cluster)
   int cta_rows;   // 256: a CTA works on two row tiles side by side; 128: on one (more CTAs when there are few rows)
+  // KV4 only
+  const uint8_t *k_codes, *v_codes;
+  const uint16_t *k_words, *v_words;
+  int head_dim, pages;
+  long long tokens;       // rows of q and out
 };
 
+// What the three producer warps of a CTA do (KV4; a fourth would leave the softmax's 64 scores a thread too few registers); `id` is 0..95 of
+// their threads. A thread takes 32 dimensions (16 bytes of codes, one group) of some keys and values of every tile. It copies them with cp.async into places of shared memory that are its own, kKv4Ahead tiles ahead, so
+// nobody has to be told when they have landed; their pages it looks up another tile ahead.
+constexpr int kKv4Producers = 96, kKv4Ahead = 3;
+constexpr int kKv4RawBytes = 40;                                  // of a thread's key and value: two times 16 bytes of codes and two words
+template <int DH> constexpr int kv4_rounds() { return (kKeysPerTile * DH / 32 + kKv4Producers - 1) / kKv4Producers; }
+template <int DH> constexpr int kv4_raw_bytes() { return kKv4Ahead * kv4_rounds<DH>() * kKv4Producers * kKv4RawBytes; }
 template <int DH, int STAGES>
-__global__ void __launch_bounds__(kUmmaAttnThreads, 1)
+__device__ __forceinline__ void kv4_produce(const UmmaPromptArgs& a, uint8_t* ring, uint8_t* raw, uint64_t* kv_full, uint64_t* kv_empty, volatile int* abort_flag,
+                                            int id, int seq, int kvh, int kt_first, int n_tiles, int lo, int hi) {
+  constexpr int GROUPS = DH / 32, PER = kv4_rounds<DH>();         // groups of a key; keys (and values) of a thread
+  constexpr int PLANE_BYTES = DH / 64 * 64 * 128, RAW = PER * kKv4Producers * kKv4RawBytes;
+  static_assert(kKv4Producers % GROUPS == 0, "a thread's keys have one group");
+  const int group = id % GROUPS, first = id / GROUPS;            // keys first + j * STEP of a tile, below its 64
+  constexpr int STEP = kKv4Producers / GROUPS;
+  const int* table = a.block_tables + static_cast<long long>(seq) * a.max_blocks;
+  const uint32_t signs = kv4_signs();
+  int rows[PER];                  // of the tile that is copied next; what no row sees is row 0, and masked below
+  const auto find = [&](int i) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int key = (kt_first + i) * kKeysPerTile + first + j * STEP;
+      rows[j] = 0;
+      if (i >= n_tiles || first + j * STEP >= kKeysPerTile || key < lo || key > hi) continue;
+      const int idx = a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size;
+      const int page = idx < a.max_blocks ? table[idx] : -1;
+      if (page < 0 || page >= a.pages) *reinterpret_cast<volatile int*>(a.status) = kStatusBadPage;
+      else rows[j] = (page * a.kv_heads + kvh - idx) * a.page_size + key;
+    }
+  };
+  const auto copy = [&](int i) {
+    if (i < n_tiles) {
+      const uint32_t dst = smem_u32(raw + (i % kKv4Ahead) * RAW);
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        if (first + j * STEP >= kKeysPerTile) break;
+        const long long at = static_cast<long long>(rows[j]) * GROUPS + group;
+        const uint32_t codes = dst + (j * kKv4Producers + id) * 32, words = dst + PER * kKv4Producers * 32 + (j * kKv4Producers + id) * 8;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(codes), "l"(a.k_codes + at * 16) : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(codes + 16), "l"(a.v_codes + at * 16) : "memory");
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(words), "l"(a.k_words + (at & ~1LL)) : "memory");          // two groups' words
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(words + 4), "l"(a.v_words + (at & ~1LL)) : "memory");
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  const auto put = [&](uint8_t* plane, int row, const uint4& codes, uint32_t words) {
+    const Kv4Scale s = kv4_scale(__byte_perm(words, 0, (group & 1) ? 0x3232 : 0x1010), signs);
+    const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
+    uint8_t* dst = plane + (group >> 1) * (64 * 128) + row * 128;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const uint32_t next = w[c] >> 8;
+      *reinterpret_cast<uint4*>(dst + ((((group & 1) * 4 + c) ^ (row & 7)) << 4)) =
+          make_uint4(kv4_low(w[c], s), kv4_high(w[c], s), kv4_low(next, s), kv4_high(next, s));
+    }
+  };
+  find(0);
+#pragma unroll 1
+  for (int i = 0; i < kKv4Ahead; ++i) {
+    copy(i);
+    find(i + 1);
+  }
+#pragma unroll 1
+  for (int i = 0; i < n_tiles; ++i) {
+    const int st = i % STAGES;
+    asm volatile("cp.async.wait_group %0;" ::"n"(kKv4Ahead - 1) : "memory");
+    const uint8_t* src = raw + (i % kKv4Ahead) * RAW;
+    uint4 kc[PER], vc[PER];
+    uint2 words[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int key = (kt_first + i) * kKeysPerTile + first + j * STEP;
+      if (first + j * STEP >= kKeysPerTile) break;
+      kc[j] = *reinterpret_cast<const uint4*>(src + (j * kKv4Producers + id) * 32);
+      vc[j] = *reinterpret_cast<const uint4*>(src + (j * kKv4Producers + id) * 32 + 16);
+      words[j] = *reinterpret_cast<const uint2*>(src + PER * kKv4Producers * 32 + (j * kKv4Producers + id) * 8);
+      if (key < lo || key > hi) words[j] = make_uint2(0u, 0u);       // what no row sees: zeros
+    }
+    copy(i + kKv4Ahead);          // (this thread's own place, whose words it holds)
+    find(i + kKv4Ahead + 1);
+    if (!__all_sync(0xffffffffu, mbar_wait(kv_empty + st, ((i / STAGES) & 1) ^ 1, abort_flag, a.status, 11) ? 1 : 0)) break;
+    uint8_t* k_plane = ring + st * 2 * PLANE_BYTES;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      if (first + j * STEP >= kKeysPerTile) break;
+      put(k_plane, first + j * STEP, kc[j], words[j].x);
+      put(k_plane + PLANE_BYTES, first + j * STEP, vc[j], words[j].y);
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if ((id & 31) == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(kv_full + st)) : "memory");
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+template <int DH, int STAGES, bool KV4>
+__global__ void __launch_bounds__(KV4 ? kUmmaKv4Threads : kUmmaAttnThreads, 1)
 attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, UmmaPromptArgs a) {
   pdl_sync();
   constexpr int HALVES = DH / 64;
@@ -70,7 +180,8 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* p_smem = smem;                 // [row tile][buffer]
   uint8_t* ring = p_smem + 4 * P_BYTES;
-  uint64_t* kv_full = reinterpret_cast<uint64_t*>(ring + STAGES * STAGE_BYTES);
+  uint8_t* raw = ring + STAGES * STAGE_BYTES;      // KV4: codes and words on their way
+  uint64_t* kv_full = reinterpret_cast<uint64_t*>(raw + (KV4 ? kv4_raw_bytes<DH>() : 0));
   uint64_t* kv_empty = kv_full + STAGES;
   uint64_t* s_full = kv_empty + STAGES;   // [2]
   uint64_t* s_empty = s_full + 2;
@@ -98,7 +209,7 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
     has[q] = r0 < rows && 128 * q < a.cta_rows;
     const int lo_pos = pos0 + r0 / G, hi_pos = pos0 + min(rows - 1, r0 + 127) / G;
     first[q] = a.window > 0 ? max(0, lo_pos - a.window + 1) / kKeysPerTile : 0;
-    last[q] = hi_pos / kKeysPerTile;
+    last[q] = (KV4 ? max(hi_pos, 0) : hi_pos) / kKeysPerTile;
   }
   int kt_first = first[0], kt_last = has[1] ? last[1] : last[0];
   if (a.splits > 1) {             // this CTA's share of the key tiles
@@ -116,7 +227,7 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(kv_full + s, 1);
+      mbar_init(kv_full + s, KV4 ? kKv4Producers / 32 : 1);
       mbar_init(kv_empty + s, 1);
     }
     for (int q = 0; q < 2; ++q) {
@@ -142,17 +253,23 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
     // Q: every softmax thread puts its own row into tensor memory (rows beyond the sequence: zeros)
     const int q = warp >> 2, rr = (warp & 3) * 32 + lane;
     const int row = row0 + 128 * q + rr;
-    const uint4* src = row < rows ? reinterpret_cast<const uint4*>(a.q + static_cast<long long>(t0 + row / G) * a.q_stride +
-                                                                  static_cast<long long>(kvh * G + row % G) * DH)
-                                  : nullptr;
+    const int head_dim = KV4 ? a.head_dim : DH;
+    const uint4* src = row < rows && (!KV4 || t0 + row / G < a.tokens)
+                           ? reinterpret_cast<const uint4*>(a.q + static_cast<long long>(t0 + row / G) * a.q_stride + static_cast<long long>(kvh * G + row % G) * head_dim)
+                           : nullptr;
     const uint32_t q_tmem = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16) + Q_COL + q * (DH / 2);
 #pragma unroll
     for (int c0 = 0; c0 < DH / 2; c0 += 16) {
       uint32_t w[16];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const uint4 v = src ? src[c0 / 4 + e] : make_uint4(0u, 0u, 0u, 0u);
-        w[4 * e] = v.x, w[4 * e + 1] = v.y, w[4 * e + 2] = v.z, w[4 * e + 3] = v.w;
+        const uint4 v = src && (!KV4 || 2 * c0 + 8 * e < head_dim) ? src[c0 / 4 + e] : make_uint4(0u, 0u, 0u, 0u);
+        if constexpr (KV4) {        // dimensions 0 4 1 5 2 6 3 7
+          w[4 * e] = __byte_perm(v.x, v.z, 0x5410), w[4 * e + 1] = __byte_perm(v.x, v.z, 0x7632);
+          w[4 * e + 2] = __byte_perm(v.y, v.w, 0x5410), w[4 * e + 3] = __byte_perm(v.y, v.w, 0x7632);
+        } else {
+          w[4 * e] = v.x, w[4 * e + 1] = v.y, w[4 * e + 2] = v.z, w[4 * e + 3] = v.w;
+        }
       }
       tmem_st16(q_tmem + c0, w);
     }
@@ -162,7 +279,10 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 
-  if (warp == 8) {
+  if (KV4 && warp != 9 && warp >= 8) {
+    const int hi = pos0 + min(rows - 1, row0 + a.cta_rows - 1) / G, lo = a.window > 0 ? max(0, pos0 + row0 / G - a.window + 1) : 0;
+    kv4_produce<DH, STAGES>(a, ring, raw, kv_full, kv_empty, abort_flag, (warp == 8 ? 0 : warp - 9) * 32 + lane, seq, kvh, kt_first, n_tiles, lo, hi);
+  } else if (!KV4 && warp == 8) {
     // ---- producer
     const int box_rows = min(a.page_size, kKeysPerTile);
     const int boxes_per_tile = kKeysPerTile / box_rows;
@@ -400,8 +520,9 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
       sums[DH] = mine ? m_used : -INFINITY;
       sums[DH + 1] = mine ? l : 0.0f;
     } else if (mine) {
-      const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-      __nv_bfloat16* o_row = row < rows ? a.out + (static_cast<long long>(t0 + row / G) * a.q_heads + kvh * G + row % G) * DH : nullptr;
+      const float inv = KV4 ? (l == 0.0f ? 0.0f : kKv4Unscale / l) : l > 0.0f ? 1.0f / l : 0.0f;
+      const int head_dim = KV4 ? a.head_dim : DH;
+      __nv_bfloat16* o_row = row < rows && (!KV4 || t0 + row / G < a.tokens) ? a.out + (static_cast<long long>(t0 + row / G) * a.q_heads + kvh * G + row % G) * head_dim : nullptr;
 #pragma unroll 1
       for (int c0 = 0; c0 < DH; c0 += 16) {
         uint32_t o[16];
@@ -410,9 +531,12 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
         if (o_row) {
           uint32_t w[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) w[e] = pack_bf16(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
-          *reinterpret_cast<uint4*>(o_row + c0) = make_uint4(w[0], w[1], w[2], w[3]);
-          *reinterpret_cast<uint4*>(o_row + c0 + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+          for (int e = 0; e < 8; ++e) {
+            const int c = KV4 ? ordered(2 * e) : 2 * e, d = KV4 ? ordered(2 * e + 1) : 2 * e + 1;
+            w[e] = pack_bf16(__uint_as_float(o[c]) * inv, __uint_as_float(o[d]) * inv);
+          }
+          if (!KV4 || c0 < head_dim) *reinterpret_cast<uint4*>(o_row + c0) = make_uint4(w[0], w[1], w[2], w[3]);
+          if (!KV4 || c0 + 8 < head_dim) *reinterpret_cast<uint4*>(o_row + c0 + 8) = make_uint4(w[4], w[5], w[6], w[7]);
         }
       }
     }
@@ -448,10 +572,11 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
         f[r] = f[r] == -INFINITY ? l[r] : ex2(f[r] - top);      // (-inf with a row sum: that is NaN)
         if (!left_out[r]) total = fmaf(l[r], f[r], total);
       }
-      const float inv = total > 0.0f ? 1.0f / total : 0.0f;
+      const float inv = KV4 ? (total == 0.0f ? 0.0f : kKv4Unscale / total) : total > 0.0f ? 1.0f / total : 0.0f;
       const int cols = DH / a.splits;
-      if (row < rows) {
-        __nv_bfloat16* dst = a.out + (static_cast<long long>(t0 + row / G) * a.q_heads + kvh * G + row % G) * DH;
+      const int head_dim = KV4 ? a.head_dim : DH;
+      if (row < rows && (!KV4 || t0 + row / G < a.tokens)) {
+        __nv_bfloat16* dst = a.out + (static_cast<long long>(t0 + row / G) * a.q_heads + kvh * G + row % G) * head_dim;
         for (int c = rank * cols; c < (rank + 1) * cols; c += 8) {
           float v[8] = {};
 #pragma unroll
@@ -467,8 +592,8 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
           }
           uint32_t w[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) w[e] = pack_bf16(v[2 * e], v[2 * e + 1]);
-          *reinterpret_cast<uint4*>(dst + c) = make_uint4(w[0], w[1], w[2], w[3]);
+          for (int e = 0; e < 4; ++e) w[e] = pack_bf16(v[KV4 ? ordered(2 * e) : 2 * e], v[KV4 ? ordered(2 * e + 1) : 2 * e + 1]);
+          if (!KV4 || c < head_dim) *reinterpret_cast<uint4*>(dst + c) = make_uint4(w[0], w[1], w[2], w[3]);
         }
       }
     }
@@ -488,15 +613,15 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
   }
 }
 
-template <int DH>
+template <int DH, bool KV4>
 static int launch_prompt_umma(const CUtensorMap& km, const CUtensorMap& vm, const UmmaPromptArgs& a, int n_seqs, int max_rows,
                               cudaStream_t s) {
-  constexpr int STAGES = DH == 128 ? 4 : 6;
-  constexpr size_t smem = 4 * 128 * 128 + static_cast<size_t>(STAGES) * 2 * (DH / 64) * 64 * 128 + (2 * STAGES + 12) * 8 + 16 + 1024;
+  constexpr int STAGES = DH == 128 ? (KV4 ? 3 : 4) : 6, THREADS = KV4 ? kUmmaKv4Threads : kUmmaAttnThreads;
+  constexpr size_t smem = 4 * 128 * 128 + static_cast<size_t>(STAGES) * 2 * (DH / 64) * 64 * 128 + (KV4 ? kv4_raw_bytes<DH>() : 0) + (2 * STAGES + 12) * 8 + 16 + 1024;
   static_assert(smem <= 227 * 1024, "shared memory of one CTA");
   static bool configured = false;
   if (!configured) {
-    if (cudaFuncSetAttribute(attn_prompt_umma_kernel<DH, STAGES>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess) {
+    if (cudaFuncSetAttribute(attn_prompt_umma_kernel<DH, STAGES, KV4>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess) {
       set_error("attention_prompt_umma: cannot reserve %zu bytes of shared memory", smem);
       return kCudaError;
     }
@@ -505,13 +630,13 @@ static int launch_prompt_umma(const CUtensorMap& km, const CUtensorMap& vm, cons
   static_assert(smem >= 256 * (DH + 4) * 4 + (2 * STAGES + 12) * 8 + 16 + 1024, "the sums of a CTA's rows");
   const dim3 grid(a.kv_heads, ceil_div(max_rows, a.cta_rows), n_seqs * a.splits);
   if (a.splits == 1) {
-    TIE_LAUNCH((attn_prompt_umma_kernel<DH, STAGES>), grid, kUmmaAttnThreads, smem, s, km, vm, a);
+    TIE_LAUNCH((attn_prompt_umma_kernel<DH, STAGES, KV4>), grid, THREADS, smem, s, km, vm, a);
     return kOk;
   }
   // clusters of CTAs that hold tensor memory are not started beside the kernel ahead
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
-  cfg.blockDim = dim3(kUmmaAttnThreads);
+  cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr;
@@ -521,8 +646,27 @@ static int launch_prompt_umma(const CUtensorMap& km, const CUtensorMap& vm, cons
   attr.val.clusterDim.z = a.splits;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, attn_prompt_umma_kernel<DH, STAGES>, km, vm, a);
+  cudaLaunchKernelEx(&cfg, attn_prompt_umma_kernel<DH, STAGES, KV4>, km, vm, a);
   return kOk;
+}
+
+// How the rows and keys of a launch are shared out over its CTAs.
+static void cut_prompt_umma(UmmaPromptArgs& a, int max_queries, int n_seqs, int max_keys) {
+  const int max_rows = max_queries * (a.q_heads / a.kv_heads);
+  // Few rows: with two row tiles a CTA, half of the SMs or more would have none
+  int sms = 148;
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, 0);
+  // ...; with many keys they share out the keys instead: what bounds either is the keys and values that L2 feeds the SMs, and tiles of
+  // 256 rows read them half as often. 128 rows a CTA against shares, us: two shares, 512 tokens of 32 heads over 8, heads of 128: 2,100
+  // keys 45 / 43, 3,000 57 / 51, 8,192 131 / 100, 16,384 246 / 175 (at 1,024 24 / 29: the merge costs about 8 us); heads of 64 37 / 37,
+  // 47 / 45, 111 / 92, 207 / 164. Four shares, 128 tokens: heads of 128 2,100 keys 43 / 37, 3,000 55 / 41, 8,192 126 / 65; 16 heads of 64 over
+  // 4 35 / 31, 45 / 35, 104 / 57; 8 over 8 of 128 41 / 29, 53 / 31, 124 / 49.
+  const long long ctas = static_cast<long long>(a.kv_heads) * ceil_div(max_rows, 256) * n_seqs;
+  const int keys = a.window > 0 && a.window + max_queries < max_keys ? a.window + max_queries : max_keys;
+  if (ctas * 2 <= sms) {
+    if (keys >= kUmmaSplitKeys) a.splits = ctas * 4 <= sms ? 4 : 2;
+    else a.cta_rows = 128;
+  }
 }
 
 }  // namespace tie
@@ -557,21 +701,39 @@ TIE_API int tie_attention_prompt_umma(const void* q, long long q_stride, const v
   UmmaPromptArgs a{static_cast<const __nv_bfloat16*>(q), static_cast<__nv_bfloat16*>(out), query_start, context_lens, block_tables,
                    status_word(), q_stride, max_blocks, q_heads, kv_heads, page_size, shift, window, scale * 1.4426950408889634f, 1, 256};
   const int max_rows = max_queries * (q_heads / kv_heads);
-  // Few rows: with two row tiles a CTA, half of the SMs or more would have none
-  int sms = 148;
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, 0);
-  // ...; with many keys they share out the keys instead: what bounds either is the keys and values that L2 feeds the SMs, and tiles of
-  // 256 rows read them half as often. 128 rows a CTA against shares, us: two shares, 512 tokens of 32 heads over 8, heads of 128: 2,100
-  // keys 45 / 43, 3,000 57 / 51, 8,192 131 / 100, 16,384 246 / 175 (at 1,024 24 / 29: the merge costs about 8 us); heads of 64 37 / 37,
-  // 47 / 45, 111 / 92, 207 / 164. Four shares, 128 tokens: heads of 128 2,100 keys 43 / 37, 3,000 55 / 41, 8,192 126 / 65; 16 heads of 64 over
-  // 4 35 / 31, 45 / 35, 104 / 57; 8 over 8 of 128 41 / 29, 53 / 31, 124 / 49.
-  const long long ctas = static_cast<long long>(kv_heads) * ceil_div(max_rows, 256) * n_seqs;
-  const int keys = window > 0 && window + max_queries < max_keys ? window + max_queries : max_keys;
-  if (ctas * 2 <= sms) {
-    if (keys >= kUmmaSplitKeys) a.splits = ctas * 4 <= sms ? 4 : 2;
-    else a.cta_rows = 128;
-  }
-  const int st = head_dim == 64 ? launch_prompt_umma<64>(km, vm, a, n_seqs, max_rows, s) : launch_prompt_umma<128>(km, vm, a, n_seqs, max_rows, s);
+  cut_prompt_umma(a, max_queries, n_seqs, max_keys);
+  const int st = head_dim == 64 ? launch_prompt_umma<64, false>(km, vm, a, n_seqs, max_rows, s) : launch_prompt_umma<128, false>(km, vm, a, n_seqs, max_rows, s);
   if (st != kOk) return st;
   TIE_RETURN_LAUNCH("attention_prompt_umma");
+}
+
+// The same over a cache in 4 bits: heads of up to 128, a multiple of 8; pages of any size; q rows 16-byte aligned.
+TIE_API int tie_attention_prompt_kv4(const void* q, long long q_stride, long long tokens, const void* k_codes, const void* k_words, const void* v_codes,
+                                     const void* v_words, void* out, const int* query_start, const int* context_lens, const int* block_tables, int max_blocks,
+                                     int n_seqs, int max_queries, int q_heads, int kv_heads, int head_dim, int page_size, long long pages, int window, float scale,
+                                     int max_keys, cudaStream_t s) {
+  TIE_REQUIRE(head_dim > 0 && head_dim <= 128 && head_dim % 8 == 0, "attention_prompt_kv4: head_dim %d is not a multiple of 8 up to 128", head_dim);
+  TIE_REQUIRE(q_heads > 0 && kv_heads > 0 && q_heads % kv_heads == 0, "attention_prompt_kv4: %d query heads over %d kv heads", q_heads, kv_heads);
+  TIE_REQUIRE(q_stride % 8 == 0 && reinterpret_cast<uintptr_t>(q) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0,
+              "attention_prompt_kv4: q and out rows must be 16-byte aligned");
+  TIE_REQUIRE(page_size > 0 && pages > 0 && pages * page_size < (1LL << 31) && max_blocks >= 0 && n_seqs >= 0 && n_seqs <= 16383 && max_queries >= 0,
+              "attention_prompt_kv4: bad sizes (%lld pages of %d, %d sequences, %d queries)", pages, page_size, n_seqs, max_queries);
+  TIE_REQUIRE(scale > 0.0f, "attention_prompt_kv4: the scale must be positive");
+  if (n_seqs == 0 || max_queries == 0) return kOk;
+  const long long all_rows = static_cast<long long>(max_queries) * (q_heads / kv_heads);
+  TIE_REQUIRE(all_rows <= 65535LL * 128, "attention_prompt_kv4: %d queries in one portion are too many", max_queries);
+  TIE_REQUIRE(status_word() != nullptr, "attention_prompt_kv4: cannot allocate the status word");
+  int shift = 0;
+  while ((1 << shift) < page_size) ++shift;
+  if ((1 << shift) != page_size) shift = -1;
+  UmmaPromptArgs a{static_cast<const __nv_bfloat16*>(q), static_cast<__nv_bfloat16*>(out), query_start, context_lens, block_tables, status_word(), q_stride, max_blocks,
+                   q_heads, kv_heads, page_size, shift, window, scale * 1.4426950408889634f * kKv4Unscale, 1, 256, static_cast<const uint8_t*>(k_codes),
+                   static_cast<const uint8_t*>(v_codes), static_cast<const uint16_t*>(k_words), static_cast<const uint16_t*>(v_words), head_dim,
+                   static_cast<int>(pages), tokens};
+  cut_prompt_umma(a, max_queries, n_seqs, max_keys);
+  const CUtensorMap none = {};
+  const int st = head_dim <= 64 ? launch_prompt_umma<64, true>(none, none, a, n_seqs, static_cast<int>(all_rows), s)
+                                : launch_prompt_umma<128, true>(none, none, a, n_seqs, static_cast<int>(all_rows), s);
+  if (st != kOk) return st;
+  TIE_RETURN_LAUNCH("attention_prompt_kv4");
 }

@@ -25,10 +25,6 @@ constexpr float kKv4LeastScale = 7.888609052210118e-31f;  // 2^-100
 constexpr int kStatusBadPage = 15;                        // a block table that names a page outside the cache, or is too short for its context
 constexpr int kStatusBadSlot = 16;                        // a slot outside the cache
 
-// Bits 4 i .. 4 i + 3 of both halves of w as two bfloat16 numbers 16 + code: the code becomes the upper four bits of the mantissa of 16.
-template <int i> __device__ __forceinline__ uint32_t kv4_pair(uint32_t w) {
-  return ((i == 0 ? w << 3 : w >> (i == 0 ? 0 : 4 * i - 3)) & 0x00780078u) | 0x41804180u;
-}
 __device__ __forceinline__ uint32_t bf16x2_mul(uint32_t a, uint32_t b) {
   uint32_t d;
   asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
@@ -39,16 +35,53 @@ __device__ __forceinline__ uint32_t bf16x2_fma(uint32_t a, uint32_t b, uint32_t 
   asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
   return d;
 }
-// Of two groups' words (one in each half; the same one twice where both numbers of a pair belong to one group): their s, and -(16 + z) s,
-// so that a pair's values are fma(16 + code, s, -(16 + z) s).
+// Taking codes apart without shifts. A bfloat16 pattern whose exponent field is 0 or 1 is its lower eight bits as a whole number times 2^-133:
+// subnormal numbers and the first normal ones lie on one line. So a code in bits 0..3 or 4..7 of a half word is a number as it stands, once
+// the other bits are masked away, code 2^-133 or code 2^-129, and one fma with s 2^69 or s 2^65 and -z s 2^-64 makes the value times 2^-64
+// of it, exactly (the products take 2^64 back in float). Against the code put into the mantissa of 16, which takes a shift and two
+// constants: a decode step over 8 x 32,768 keys KV4_US us against 94; logical operations and shifts share the pipe that bounds these kernels.
+// Scales from 2^57 up count as 2^57, so that s 2^69 stays finite (and NaN stays NaN); values below 2^-62 lose bits.
+constexpr float kKv4Unscale = 18446744073709551616.0f;     // 2^64
+// `words`: two groups' words, one in each half (the same one twice where both numbers of a pair belong to one group).
 struct Kv4Scale {
-  uint32_t s, off;
+  uint32_t low, high, off;      // for codes in bits 0..3 and 4..7; -z s 2^-64
 };
-__device__ __forceinline__ Kv4Scale kv4_scale(uint32_t words) {
+// (signs: two sign bits, in a register: with a constant the compiler makes two operations of the and-or)
+__device__ __forceinline__ uint32_t kv4_signs() {
+  uint32_t signs;
+  asm volatile("mov.b32 %0, 0x80008000;" : "=r"(signs));
+  return signs;
+}
+__device__ __forceinline__ Kv4Scale kv4_scale(uint32_t words, uint32_t signs) {
   Kv4Scale k;
-  k.s = words & 0xffe0ffe0u;
-  k.off = bf16x2_mul(((words & 0x000f000fu) << 3) | 0xc180c180u, k.s);
+  uint32_t z;
+  asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(k.low) : "r"(words & 0xffe0ffe0u), "r"(0x5c005c00u));     // 2^57
+  k.low = bf16x2_mul(k.low, 0x62006200u);                                                           // 2^69
+  k.high = bf16x2_mul(k.low, 0x3d803d80u);                                                          // 2^-4
+  asm("lop3.b32 %0, %1, 0x000f000f, %2, 0xEA;" : "=r"(z) : "r"(words), "r"(signs));                  // -z 2^-133
+  k.off = bf16x2_mul(z, k.low);
   return k;
+}
+// The values 2^-64 of the codes in bits 0..3 (4..7) of both halves of w.
+__device__ __forceinline__ uint32_t kv4_low(uint32_t w, const Kv4Scale& k) { return bf16x2_fma(w & 0x000f000fu, k.low, k.off); }
+__device__ __forceinline__ uint32_t kv4_high(uint32_t w, const Kv4Scale& k) { return bf16x2_fma(w & 0x00f000f0u, k.high, k.off); }
+
+// Eight dimensions of a row, `dims` of them there (the others are zero); vec: rows are 16-byte aligned.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int dims, bool vec, float (&x)[8]) {
+  if (vec && dims >= 8) {
+    constexpr int N = Vec16<T>::N;
+#pragma unroll
+    for (int i = 0; i < 8; i += N) {
+      Vec16<T> t;
+      t.load(p + i);
+#pragma unroll
+      for (int e = 0; e < N; ++e) x[i + e] = t.v[e];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = i < dims ? ld(p + i) : 0.0f;
+  }
 }
 
 // The smallest number of three significant bits that is not below (hi - lo) / 15; the float division rounds first.

@@ -21,23 +21,6 @@ __device__ __forceinline__ long long kv4_row(int slot, int head, int kv_heads, i
   return (static_cast<long long>(slot / page_size) * kv_heads + head) * page_size + slot % page_size;
 }
 
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, int dims, bool vec, float (&x)[8]) {
-  if (vec && dims >= 8) {
-    constexpr int N = Vec16<T>::N;
-#pragma unroll
-    for (int i = 0; i < 8; i += N) {
-      Vec16<T> t;
-      t.load(p + i);
-#pragma unroll
-      for (int e = 0; e < N; ++e) x[i + e] = t.v[e];
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = i < dims ? ld(p + i) : 0.0f;
-  }
-}
-
 // NG: head_dim in 64s. Up to two a key and value fit a warp's lanes side by side (one: half a warp), else the lanes hold a word of both.
 template <typename T, int NG>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const T* __restrict__ k, const T* __restrict__ v, long long k_stride, long long v_stride,

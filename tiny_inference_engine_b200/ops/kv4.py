@@ -66,32 +66,37 @@ class StepArrays(NamedTuple):
 TABLES_NO_PAGES, TABLES_SHORT, TABLES_ROWS, TABLES_BAD_REQUEST = 1, 2, 4, 8
 
 
+# The checks run on every call, ahead of kernels of a few microseconds: conditions are tested in plain `if`s, so that a message is only put
+# together when it is needed, and every property of a tensor is asked for once.
+
 def _need(cond, msg: str) -> None:
     if not cond:
         raise InvalidArgument(msg)
 
 
-def _one_device(what: str, *ts) -> None:
+def _fail(msg: str):
+    raise InvalidArgument(msg)
+
+
+UMMA_MIN_ROWS = 128     # rows (queries x heads of a group) from which the tcgen05 kernel takes a portion of a prompt
+_FLOATS = {torch.float32: 0, torch.bfloat16: 1}
+_I32 = torch.int32
+
+
+def _stream(what: str, *ts) -> int:
+    """The current stream, once every tensor is known to be on the current device."""
+    here = torch._C._cuda_getDevice() if ts[0].is_cuda else -1
     for t in ts:
-        if t is not None and not t.is_cuda:
-            raise InvalidArgument("kernel arguments must be CUDA tensors: the engine has no CPU path")
-    devices = {t.device for t in ts if t is not None}
-    _need(len(devices) == 1 and next(iter(devices)).index == torch.cuda.current_device(),
-          f"{what}: all tensors must be on the current device, got {sorted(map(str, devices))}")
+        if t.get_device() != here or here < 0:
+            _fail("kernel arguments must be CUDA tensors: the engine has no CPU path" if not t.is_cuda else
+                  f"{what}: all tensors must be on the current device, {here}, got one on {t.device}")
+    return torch._C._cuda_getCurrentRawStream(here)
 
 
-def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
-
-
-def _int32(what: str, name: str, t, *shape) -> None:
-    _need(t.dtype == torch.int32 and t.is_contiguous() and tuple(t.shape) == shape, f"{what}: {name} must be contiguous int32 {list(shape)}")
-
-
-def _float_code(what: str, *ts) -> int:
-    codes = {torch.float32: 0, torch.bfloat16: 1}
-    _need(ts[0].dtype in codes and all(t.dtype == ts[0].dtype for t in ts), f"{what}: rows must be float32 or bfloat16, all alike")
-    return codes[ts[0].dtype]
+def _int32(what: str, name: str, t, n: int) -> None:
+    """A contiguous vector of n int32 numbers."""
+    if t.dtype is not _I32 or t.numel() != n or not t.is_contiguous():
+        _fail(f"{what}: {name} must be contiguous int32 [{n}]")
 
 
 def kv4_cache(pages: int, kv_heads: int, page_size: int, head_dim: int, device="cuda") -> Kv4Cache:
@@ -105,84 +110,122 @@ def kv4_cache(pages: int, kv_heads: int, page_size: int, head_dim: int, device="
     return Kv4Cache(plane(padded // 2, torch.uint8), plane(padded // 32, torch.int16), plane(padded // 2, torch.uint8), plane(padded // 32, torch.int16), head_dim)
 
 
-def _check_cache(what: str, c: Kv4Cache) -> None:
-    _need(0 < c.head_dim <= 256, f"{what}: head size {c.head_dim} is not in 1..256")
-    padded = -(-c.head_dim // 64) * 64
-    for codes, words in ((c.k_codes, c.k_words), (c.v_codes, c.v_words)):
-        _need(codes.dim() == 4 and codes.dtype == torch.uint8 and codes.shape[3] == padded // 2 and words.dtype == torch.int16 and
-              tuple(words.shape) == (*codes.shape[:3], padded // 32) and codes.shape == c.k_codes.shape and codes.is_contiguous() and words.is_contiguous(),
-              f"{what}: planes must be contiguous, codes uint8 [pages, kv_heads, page_size, {padded // 2}] and words int16 [..., {padded // 32}]")
-        _need(codes.data_ptr() % 16 == 0 and words.data_ptr() % 16 == 0, f"{what}: planes must be 16-byte aligned")
-    _need(c.pages > 0 and c.kv_heads > 0 and c.page_size > 0 and c.pages * c.page_size < 2 ** 31, f"{what}: slots must be 32-bit numbers, of one page at least")
+def _check_cache(what: str, c: Kv4Cache) -> tuple:
+    """The planes' addresses and (kv heads, head size, page size, pages)."""
+    kc, kw, vc, vw, dim = c
+    if not 0 < dim <= 256:
+        _fail(f"{what}: head size {dim} is not in 1..256")
+    words = (dim + 63) // 64 * 2
+    shape = kc.shape
+    if len(shape) != 4:
+        _fail(f"{what}: codes must be [pages, kv_heads, page_size, bytes]")
+    pages, heads, size, width = shape
+    n = pages * heads * size * words
+    if width != 16 * words or not (kc.dtype is vc.dtype is torch.uint8 and kw.dtype is vw.dtype is torch.int16) or kw.numel() != n or vw.numel() != n or \
+            vc.numel() != 16 * n or not (kc.is_contiguous() and kw.is_contiguous() and vc.is_contiguous() and vw.is_contiguous()):
+        _fail(f"{what}: planes must be contiguous, codes uint8 [pages, kv_heads, page_size, {16 * words}] and words int16 [..., {words}]")
+    if n == 0 or pages * size >= 2 ** 31:
+        _fail(f"{what}: slots must be 32-bit numbers, of one page at least")
+    planes = kc.data_ptr(), kw.data_ptr(), vc.data_ptr(), vw.data_ptr()
+    if (planes[0] | planes[1] | planes[2] | planes[3]) & 15:
+        _fail(f"{what}: planes must be 16-byte aligned")
+    return planes, (heads, dim, size, pages)
 
 
-def _check_rows(what: str, c: Kv4Cache, k, v, slots) -> int:
-    _check_cache(what, c)
-    dtype = _float_code(what, k, v)
-    _need(k.dim() == 2 and k.shape == v.shape and k.shape[1] == c.kv_heads * c.head_dim and all(t.stride(1) == 1 or t.shape[1] == 1 for t in (k, v)),
-          f"{what}: k and v must be [T, {c.kv_heads * c.head_dim}] with contiguous rows")
-    _int32(what, "slots", slots, k.shape[0])
-    _one_device(what, k, v, slots, *c[:4])
-    return dtype
+def _check_rows(what: str, c: Kv4Cache, k, v, slots) -> tuple:
+    planes, sizes = _check_cache(what, c)
+    dtype = _FLOATS.get(k.dtype)
+    if dtype is None or v.dtype is not k.dtype:
+        _fail(f"{what}: rows must be float32 or bfloat16, all alike")
+    shape, width = k.shape, sizes[0] * sizes[1]
+    if len(shape) != 2 or shape[1] != width or v.shape != shape:
+        _fail(f"{what}: k and v must be [T, {width}]")
+    (k_stride, k_step), (v_stride, v_step) = k.stride(), v.stride()
+    if (k_step != 1 or v_step != 1) and width > 1:
+        _fail(f"{what}: k and v must be [T, {width}] with contiguous rows")
+    _int32(what, "slots", slots, shape[0])
+    return dtype, planes, sizes, shape[0], k_stride, v_stride, _stream(what, k, v, slots, c[0], c[1], c[2], c[3])
 
 
 def kv4_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: Kv4Cache) -> None:
     """k, v [T, kv_heads * head_dim] (float32 or bfloat16, rows may be strided) into the cache at slots[t]; slot < 0 writes nothing. The slots of a
     call must differ: of a slot that is named twice it is not said which row it keeps, or which part of either. A slot outside of the cache
     writes nothing either and is reported by `gemm_select.check_status`."""
-    dtype = _check_rows("kv4_append", cache, k, v, slots)
-    call("tie_kv4_append", dtype, k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0), slots.data_ptr(), cache.k_codes.data_ptr(),
-         cache.k_words.data_ptr(), cache.v_codes.data_ptr(), cache.v_words.data_ptr(), k.shape[0], cache.kv_heads, cache.head_dim, cache.page_size,
-         cache.pages, _stream())
+    dtype, planes, sizes, T, k_stride, v_stride, stream = _check_rows("kv4_append", cache, k, v, slots)
+    call("tie_kv4_append", dtype, k.data_ptr(), v.data_ptr(), k_stride, v_stride, slots.data_ptr(), *planes, T, *sizes, stream)
 
 
 def kv4_read(cache: Kv4Cache, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
     """The values that the cache holds at slots[t] into k, v [T, kv_heads * head_dim] (float32 or bfloat16, exact in both); rows whose slot is below
     zero are left as they are."""
-    dtype = _check_rows("kv4_read", cache, k, v, slots)
-    call("tie_kv4_read", dtype, cache.k_codes.data_ptr(), cache.k_words.data_ptr(), cache.v_codes.data_ptr(), cache.v_words.data_ptr(), slots.data_ptr(),
-         k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0), k.shape[0], cache.kv_heads, cache.head_dim, cache.page_size, cache.pages, _stream())
+    dtype, planes, sizes, T, k_stride, v_stride, stream = _check_rows("kv4_read", cache, k, v, slots)
+    call("tie_kv4_read", dtype, *planes, slots.data_ptr(), k.data_ptr(), v.data_ptr(), k_stride, v_stride, T, *sizes, stream)
 
 
 def kv4_workspace(q_heads: int, kv_heads: int, head_dim: int, device="cuda") -> Kv4Workspace:
     """The workspace of `attention_kv4_decode` and `attention_kv4_prompt` for heads of these sizes, whatever the batch."""
     _need(q_heads > 0 and kv_heads > 0 and q_heads % kv_heads == 0 and 0 < head_dim <= 256, "kv4_workspace: bad sizes")
     ctas = library().tie_attention_kv4_ctas()
-    return Kv4Workspace(torch.empty(ctas * 16 * (head_dim + 2), dtype=torch.float32, device=device), torch.zeros(ctas, dtype=torch.int32, device=device))
+    return Kv4Workspace(torch.empty(ctas * 16 * (-(-head_dim // 64) * 64 + 2), dtype=torch.float32, device=device), torch.zeros(ctas, dtype=torch.int32, device=device))
 
 
-def _check_attention(what, q, cache, out, query_start, context_lens, block_tables, q_heads, workspace, window, n: int, scale,
-                     max_context, max_queries: int, seq_list=None) -> int:
-    _check_cache(what, cache)
-    dtype = _float_code(what, q, out)
-    _need(q_heads > 0 and q_heads % cache.kv_heads == 0, f"{what}: {q_heads} heads are not a multiple of {cache.kv_heads} kv heads")
-    width = q_heads * cache.head_dim
-    _need(q.dim() == 2 and q.shape[1] >= width and (q.stride(1) == 1 or q.shape[1] == 1), f"{what}: q must be [T, {width}] or wider, with contiguous rows")
-    _need(tuple(out.shape) == (q.shape[0], width) and out.is_contiguous(), f"{what}: out must be contiguous [T, {width}]")
+def _workspace_ctas() -> int:
+    global _CTAS
+    if _CTAS is None:
+        _CTAS = library().tie_attention_kv4_ctas()
+    return _CTAS
+
+
+_CTAS = None        # CTAs that may leave partial sums: what the kernels were compiled for
+
+
+def _check_attention(what, q, cache, out, query_start, context_lens, block_tables, q_heads, workspace, window, n: int, scale, max_context,
+                     max_queries: int, seq_list=None) -> tuple:
+    """(dtype, the planes' addresses, their sizes, rows, row stride of q, sequences, columns of the block tables, stream)"""
+    planes, sizes = _check_cache(what, cache)
+    dtype = _FLOATS.get(q.dtype)
+    if dtype is None or out.dtype is not q.dtype:
+        _fail(f"{what}: rows must be float32 or bfloat16, all alike")
+    if q_heads <= 0 or q_heads % sizes[0]:
+        _fail(f"{what}: {q_heads} heads are not a multiple of {sizes[0]} kv heads")
+    width, shape, out_shape, table_shape = q_heads * sizes[1], q.shape, out.shape, block_tables.shape
+    if len(shape) != 2 or shape[1] < width:
+        _fail(f"{what}: q must be [T, {width}] or wider")
+    q_stride, step = q.stride()
+    if step != 1 and shape[1] > 1:
+        _fail(f"{what}: q must have contiguous rows")
+    if len(out_shape) != 2 or out_shape[0] != shape[0] or out_shape[1] != width or not out.is_contiguous():
+        _fail(f"{what}: out must be contiguous [T, {width}]")
     S = context_lens.numel()
     _int32(what, "query_start", query_start, S + 1)
     _int32(what, "context_lens", context_lens, S)
-    _need(block_tables.dim() == 2, f"{what}: block_tables must be [sequences, pages]")
-    _int32(what, "block_tables", block_tables, S, block_tables.shape[1])
-    _need(0 <= n <= S or seq_list is not None, f"{what}: {n} of {S} sequences")
-    _need(0 <= n <= 65535, f"{what}: at most 65,535 sequences a call, got {n}")
-    _need(0 <= window < 2 ** 30, f"{what}: bad window {window}")
-    ctas = library().tie_attention_kv4_ctas()
-    _need(workspace.scratch.dtype == torch.float32 and workspace.scratch.is_contiguous() and workspace.scratch.numel() >= ctas * 16 * (cache.head_dim + 2) and
-          workspace.counters.dtype == torch.int32 and workspace.counters.is_contiguous() and workspace.counters.numel() >= ctas,
-          f"{what}: the workspace is too small (kv4_workspace makes one)")
-    _need(scale > 0 and max_context >= 0 and 0 <= max_queries < 2 ** 30, f"{what}: the scale must be positive, max_context and max_queries not negative")
-    _need(seq_list is None or (seq_list.dtype == torch.int32 and seq_list.dim() == 1 and seq_list.is_contiguous() and seq_list.numel() >= n),
-          f"{what}: seq_list must be int32 [n_list]")
-    _one_device(what, q, out, query_start, context_lens, block_tables, seq_list, *workspace, *cache[:4])
-    return dtype
+    if len(table_shape) != 2 or table_shape[0] != S or block_tables.dtype is not _I32 or not block_tables.is_contiguous():
+        _fail(f"{what}: block_tables must be contiguous int32 [{S}, pages]")
+    if not 0 <= n <= 65535 or (seq_list is None and n > S):
+        _fail(f"{what}: {n} of {S} sequences (at most 65,535 a call)")
+    if not 0 <= window < 2 ** 30:
+        _fail(f"{what}: bad window {window}")
+    scratch, counters = workspace
+    ctas = _workspace_ctas()
+    if scratch.dtype is not torch.float32 or counters.dtype is not _I32 or scratch.numel() < ctas * 16 * ((sizes[1] + 63) // 64 * 64 + 2) or scratch.data_ptr() & 15 or counters.numel() < ctas or not (
+            scratch.is_contiguous() and counters.is_contiguous()):
+        _fail(f"{what}: the workspace is too small (kv4_workspace makes one)")
+    if not (scale > 0 and max_context >= 0 and 0 <= max_queries < 2 ** 30):
+        _fail(f"{what}: the scale must be positive, max_context and max_queries not negative")
+    if seq_list is None:
+        stream = _stream(what, q, out, query_start, context_lens, block_tables, scratch, counters, cache[0], cache[1], cache[2], cache[3])
+    else:
+        if seq_list.dtype is not _I32 or seq_list.dim() != 1 or not seq_list.is_contiguous() or seq_list.numel() < n:
+            _fail(f"{what}: seq_list must be int32 [n_list]")
+        stream = _stream(what, q, out, query_start, context_lens, block_tables, scratch, counters, cache[0], cache[1], cache[2], cache[3], seq_list)
+    return dtype, planes, sizes, shape[0], q_stride, S, table_shape[1], stream
 
 
-def _rows_kernel(dtype, q, cache, out, query_start, context_lens, block_tables, max_queries, q_heads, scale, window, seq_list, n, max_context, workspace):
-    call("tie_attention_kv4", dtype, q.data_ptr(), q.stride(0), q.shape[0], cache.k_codes.data_ptr(), cache.k_words.data_ptr(), cache.v_codes.data_ptr(),
-         cache.v_words.data_ptr(), out.data_ptr(), query_start.data_ptr(), context_lens.data_ptr(), block_tables.data_ptr(), block_tables.shape[1],
-         context_lens.numel(), max_queries, q_heads, cache.kv_heads, cache.head_dim, cache.page_size, cache.pages, int(window), float(scale),
-         0 if seq_list is None else seq_list.data_ptr(), n, int(max_context), workspace.scratch.data_ptr(), workspace.counters.data_ptr(), _stream())
+def _rows_kernel(checked, q, out, query_start, context_lens, block_tables, max_queries, q_heads, scale, window, seq_list, n, max_context, workspace):
+    dtype, planes, sizes, T, q_stride, S, columns, stream = checked
+    call("tie_attention_kv4", dtype, q.data_ptr(), q_stride, T, *planes, out.data_ptr(), query_start.data_ptr(), context_lens.data_ptr(),
+         block_tables.data_ptr(), columns, S, max_queries, q_heads, *sizes, window, scale, seq_list, n, min(max_context, 2 ** 30),
+         workspace[0].data_ptr(), workspace[1].data_ptr(), stream)
 
 
 def attention_kv4_decode(q, cache: Kv4Cache, out, query_start, context_lens, block_tables, q_heads: int, scale: float, seq_list, n_list: int,
@@ -192,12 +235,10 @@ def attention_kv4_decode(q, cache: Kv4Cache, out, query_start, context_lens, blo
     float32 or bfloat16, out [T, q_heads * head_dim] alike; a sequence without keys gets zeros, other rows are left as they are.
     `max_context`: about the longest of the contexts (how the launch is cut, not what it computes), so that a captured call stays right
     as contexts grow. Softmax statistics and sums are 32-bit; the weights enter the value product with 16 bits (float32 rows: 24)."""
-    what = "attention_kv4_decode"
-    dtype = _check_attention(what, q, cache, out, query_start, context_lens, block_tables, q_heads, workspace, window, n_list, scale,
-                             max_context, 1, seq_list)
-    if n_list == 0 or q.shape[0] == 0:
-        return
-    _rows_kernel(dtype, q, cache, out, query_start, context_lens, block_tables, 1, q_heads, scale, window, seq_list, n_list, min(int(max_context), 2 ** 30), workspace)
+    checked = _check_attention("attention_kv4_decode", q, cache, out, query_start, context_lens, block_tables, q_heads, workspace, window, n_list, scale,
+                               max_context, 1, seq_list)
+    if n_list and checked[3]:
+        _rows_kernel(checked, q, out, query_start, context_lens, block_tables, 1, q_heads, scale, window, seq_list.data_ptr(), n_list, max_context, workspace)
 
 
 def attention_kv4_prompt(q, cache: Kv4Cache, out, query_start, context_lens, block_tables, n_seqs: int, max_queries: int, q_heads: int, scale: float,
@@ -205,14 +246,19 @@ def attention_kv4_prompt(q, cache: Kv4Cache, out, query_start, context_lens, blo
     """Causal attention of the first n_seqs sequences of the step, each bringing up to max_queries tokens that are in the cache already: row t of
     sequence s sits at pos = context_lens[s] - (its queries) + (t - query_start[s]) and sees keys 0..pos (with a window: the last `window` of
     them). Types, layouts and `max_context` as in `attention_kv4_decode`."""
-    what = "attention_kv4_prompt"
-    dtype = _check_attention(what, q, cache, out, query_start, context_lens, block_tables, q_heads, workspace, window, n_seqs, scale,
-                             max_context, max_queries)
-    max_queries = min(max_queries, q.shape[0])
-    if n_seqs == 0 or max_queries == 0:
+    checked = _check_attention("attention_kv4_prompt", q, cache, out, query_start, context_lens, block_tables, q_heads, workspace, window, n_seqs, scale,
+                               max_context, max_queries)
+    max_queries = min(max_queries, checked[3])
+    if not n_seqs or not max_queries:
         return
-    _rows_kernel(dtype, q, cache, out, query_start, context_lens, block_tables, max_queries, q_heads, scale, window, None, n_seqs, min(int(max_context), 2 ** 30),
-                 workspace)
+    dtype, planes, sizes, T, q_stride, _, columns, stream = checked
+    rows = max_queries * (q_heads // sizes[0])
+    if dtype == 1 and rows >= UMMA_MIN_ROWS and sizes[1] <= 128 and sizes[1] % 8 == 0 and q_stride % 8 == 0 and not (q.data_ptr() | out.data_ptr()) & 15 and \
+            n_seqs <= 16383 and rows <= 65535 * 128:
+        call("tie_attention_prompt_kv4", q.data_ptr(), q_stride, T, *planes, out.data_ptr(), query_start.data_ptr(), context_lens.data_ptr(),
+             block_tables.data_ptr(), columns, n_seqs, max_queries, q_heads, *sizes, window, scale, min(max_context, 2 ** 30), stream)
+    else:
+        _rows_kernel(checked, q, out, query_start, context_lens, block_tables, max_queries, q_heads, scale, window, 0, n_seqs, max_context, workspace)
 
 
 def step_arrays(n: int, rows: int, columns: int, device="cuda") -> StepArrays:
@@ -224,16 +270,18 @@ def step_arrays(n: int, rows: int, columns: int, device="cuda") -> StepArrays:
     return StepArrays(empty(n + 1), empty(n), empty(rows), empty(rows), empty(rows), empty(n, columns), empty(1), empty(1))
 
 
-def _check_tables(what, requests, lens, tables, free_pages, free_count, page_size) -> int:
-    _need(requests.dim() == 1 and lens.dim() == 1 and tables.dim() == 2 and free_pages.dim() == 1, f"{what}: requests, lens and free_pages must be 1-D, tables 2-D")
-    n = requests.shape[0]
+def _check_tables(what, requests, lens, tables, free_pages, free_count, page_size) -> tuple:
+    """(sequences, requests of the state, columns of its tables, pages)"""
+    shape, n, held, pages = tables.shape, requests.numel(), lens.numel(), free_pages.numel()
     _int32(what, "requests", requests, n)
-    _int32(what, "lens", lens, lens.shape[0])
-    _int32(what, "tables", tables, lens.shape[0], tables.shape[1])
-    _int32(what, "free_pages", free_pages, free_pages.shape[0])
+    _int32(what, "lens", lens, held)
+    _int32(what, "free_pages", free_pages, pages)
     _int32(what, "free_count", free_count, 1)
-    _need(page_size > 0, f"{what}: page size must be positive")
-    return n
+    if len(shape) != 2 or shape[0] != held or tables.dtype is not _I32 or not tables.is_contiguous():
+        _fail(f"{what}: tables must be contiguous int32 [{held}, pages]")
+    if page_size <= 0:
+        _fail(f"{what}: page size must be positive")
+    return n, held, shape[1], pages
 
 
 def step_tables(requests, counts, lens, tables, free_pages, free_count, page_size: int, arrays: StepArrays, commit: bool = True) -> None:
@@ -249,18 +297,24 @@ def step_tables(requests, counts, lens, tables, free_pages, free_count, page_siz
     `tables` or the block tables are wide; more rows than the arrays have; a request outside of lens, a negative count or length, a request
     named twice), every slot is -1, every context and query_start 0, and the state stays as it was."""
     what = "step_tables"
-    n = _check_tables(what, requests, lens, tables, free_pages, free_count, page_size)
-    rows, columns = arrays.slots.shape[0], arrays.block_tables.shape[-1]
+    n, held, width, pages = _check_tables(what, requests, lens, tables, free_pages, free_count, page_size)
+    query_start, context_lens, positions, seq_of_row, slots, block_tables, free_left, status = arrays
+    rows, shape = slots.numel(), block_tables.shape
     _int32(what, "counts", counts, n)
-    for name, shape in (("query_start", (n + 1,)), ("context_lens", (n,)), ("positions", (rows,)), ("seq_of_row", (rows,)), ("slots", (rows,)),
-                        ("block_tables", (n, columns)), ("free_left", (1,)), ("status", (1,))):
-        _int32(what, f"arrays.{name}", getattr(arrays, name), *shape)
-    _need(0 < columns <= tables.shape[1], f"{what}: block tables of {columns} pages, tables of {tables.shape[1]}")
-    _one_device(what, requests, counts, lens, tables, free_pages, free_count, *arrays)
+    _int32(what, "arrays.query_start", query_start, n + 1)
+    _int32(what, "arrays.context_lens", context_lens, n)
+    _int32(what, "arrays.positions", positions, rows)
+    _int32(what, "arrays.seq_of_row", seq_of_row, rows)
+    _int32(what, "arrays.slots", slots, rows)
+    _int32(what, "arrays.free_left", free_left, 1)
+    _int32(what, "arrays.status", status, 1)
+    if len(shape) != 2 or shape[0] != n or block_tables.dtype is not _I32 or not block_tables.is_contiguous() or not 0 < shape[1] <= width:
+        _fail(f"{what}: arrays.block_tables must be contiguous int32 [{n}, up to {width}]")
+    stream = _stream(what, requests, counts, lens, tables, free_pages, free_count, query_start, context_lens, positions, seq_of_row, slots, block_tables,
+                     free_left, status)
     call("tie_step_tables", requests.data_ptr(), counts.data_ptr(), lens.data_ptr(), tables.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(),
-         arrays.query_start.data_ptr(), arrays.context_lens.data_ptr(), arrays.positions.data_ptr(), arrays.seq_of_row.data_ptr(), arrays.slots.data_ptr(),
-         arrays.block_tables.data_ptr(), arrays.free_left.data_ptr(), arrays.status.data_ptr(), n, rows, columns, tables.shape[1], lens.shape[0],
-         free_pages.shape[0], page_size, 1 if commit else 0, _stream())
+         query_start.data_ptr(), context_lens.data_ptr(), positions.data_ptr(), seq_of_row.data_ptr(), slots.data_ptr(), block_tables.data_ptr(),
+         free_left.data_ptr(), status.data_ptr(), n, rows, shape[1], width, held, pages, page_size, 1 if commit else 0, stream)
 
 
 def release_tables(requests, lens, tables, free_pages, free_count, page_size: int, status) -> None:
@@ -268,8 +322,8 @@ def release_tables(requests, lens, tables, free_pages, free_count, page_size: in
     pages in theirs, as `CacheManager.release` gives them back; their lengths become 0. Refused whole, with the TABLES_* bits in `status`
     (int32 [1], else 0), where a request or length cannot be or the stack would overflow."""
     what = "release_tables"
-    n = _check_tables(what, requests, lens, tables, free_pages, free_count, page_size)
+    n, held, width, pages = _check_tables(what, requests, lens, tables, free_pages, free_count, page_size)
     _int32(what, "status", status, 1)
-    _one_device(what, requests, lens, tables, free_pages, free_count, status)
+    stream = _stream(what, requests, lens, tables, free_pages, free_count, status)
     call("tie_release_tables", requests.data_ptr(), lens.data_ptr(), tables.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(), status.data_ptr(), n,
-         lens.shape[0], tables.shape[1], free_pages.shape[0], page_size, _stream())
+         held, width, pages, page_size, stream)
