@@ -397,7 +397,9 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
     const int q = warp >> 2, wq = warp & 3;
     const int rr = wq * 32 + lane;                           // row inside the tile = lane of tensor memory
     const int row = row0 + 128 * q + rr;
-    const int pos = row < rows ? pos0 + row / G : -1;       // rows beyond the sequence see no key
+    // Rows beyond the sequence (their queries are zeros, nothing of them is written) see what its last one sees: with no key at all they would
+    // take the whole warp through the masks in every tile (portions of 512, 512, 512 and 2 tokens at 8,192 keys 344 us instead of 173).
+    const int pos = pos0 + min(row, rows - 1) / G;
     const uint32_t lane_base = static_cast<uint32_t>(wq * 32) << 16;
     const uint32_t s_tmem = tmem_base + lane_base + q * kKeysPerTile;
     const uint32_t o_tmem = tmem_base + lane_base + O_COL + q * DH;
@@ -669,6 +671,27 @@ static void cut_prompt_umma(UmmaPromptArgs& a, int max_queries, int n_seqs, int 
   }
 }
 
+// The same with KV4, by what the ways cost in tiles of 64 keys by 256 rows: the CTAs' rounds on the SMs times a CTA's tiles. Two shares of the
+// keys add the time of 8 tiles to a round, four 12 (and four CTAs of a cluster find room on about 132 of the SMs); CTAs of 128 rows take 0.86 of a
+// tile's time. How many CTAs have rows is estimated from all rows of the step, since portions differ. Against what was measured (us): portions
+// of 512, 342, 172 and 2 tokens of 16 heads of 64 over 4 at 8,192 keys: one share 172, two 97, four 153 (the rule: two); 512 tokens of
+// 32 heads of 128 over 8 at 8,192 keys 203, 115, 143 (two); 128 tokens at 4,096 keys 107, 67, 48 (four); 1,024 tokens at 4,096 keys 108, 121, 180
+// (one); eight portions of 300 to 2 tokens at 4,096 keys 198, 184, 242 (two); 300 tokens at 300 keys 18.5, 22, 43, 128 rows 16.3 (128 rows).
+static void cut_prompt_kv4(UmmaPromptArgs& a, int max_queries, int n_seqs, int max_keys) {
+  const long long group = a.q_heads / a.kv_heads, max_rows = max_queries * group;
+  const int keys = a.window > 0 && a.window + max_queries < max_keys ? a.window + max_queries : max_keys;
+  const double tiles = (keys + kKeysPerTile - 1) / kKeysPerTile;
+  double best = 0.0;
+  const int ways[4][3] = {{1, 256, 0}, {1, 128, 0}, {2, 256, 8}, {4, 256, 12}};
+  for (int i = 0; i < 4; ++i) {
+    const int splits = ways[i][0], rows = ways[i][1];
+    const long long most = n_seqs * ((max_rows + rows - 1) / rows), about = (2 * a.tokens * group + (n_seqs + 1) * rows) / (2 * rows);
+    const long long ctas = a.kv_heads * (most < about ? most : about) * splits, places = splits == 4 ? 132 : 148;
+    const double cost = static_cast<double>((ctas + places - 1) / places) * (rows == 128 ? 0.86 : 1.0) * (tiles / splits + ways[i][2]);
+    if (i == 0 || cost < best) best = cost, a.splits = splits, a.cta_rows = rows;
+  }
+}
+
 }  // namespace tie
 
 using namespace tie;
@@ -730,7 +753,7 @@ TIE_API int tie_attention_prompt_kv4(const void* q, long long q_stride, long lon
                    q_heads, kv_heads, page_size, shift, window, scale * 1.4426950408889634f * kKv4Unscale, 1, 256, static_cast<const uint8_t*>(k_codes),
                    static_cast<const uint8_t*>(v_codes), static_cast<const uint16_t*>(k_words), static_cast<const uint16_t*>(v_words), head_dim,
                    static_cast<int>(pages), tokens};
-  cut_prompt_umma(a, max_queries, n_seqs, max_keys);
+  cut_prompt_kv4(a, max_queries, n_seqs, max_keys);
   const CUtensorMap none = {};
   const int st = head_dim <= 64 ? launch_prompt_umma<64, true>(none, none, a, n_seqs, static_cast<int>(all_rows), s)
                                 : launch_prompt_umma<128, true>(none, none, a, n_seqs, static_cast<int>(all_rows), s);

@@ -12,119 +12,155 @@ int* status_word();
 struct Kv4Planes {
   uint32_t *k_codes, *v_codes;
   uint16_t *k_words, *v_words;
-  int kv_heads, page_size, head_dim;
+  int kv_heads, page_size, page_shift, head_dim;     // page_shift -1: no power of two
   unsigned int slots;       // pages * page_size
 };
 
-// Row of the planes (token slots of one head) of a slot.
-__device__ __forceinline__ long long kv4_row(int slot, int head, int kv_heads, int page_size) {
-  return (static_cast<long long>(slot / page_size) * kv_heads + head) * page_size + slot % page_size;
+// Row of the planes (token slots of one head) of a slot; a plane has less than 2^31.
+__device__ __forceinline__ int kv4_row(int slot, int head, const Kv4Planes& c) {
+  const int page = c.page_shift >= 0 ? slot >> c.page_shift : slot / c.page_size;
+  return (page * c.kv_heads + head - page) * c.page_size + slot;
 }
 
-// NG: head_dim in 64s. Up to two a key and value fit a warp's lanes side by side (one: half a warp), else the lanes hold a word of both.
-template <typename T, int NG>
+// A head's token: up to two 64s (NG) its key and value are the lanes of a warp side by side (one 64: of half a warp), else every lane has a word
+// of both. blockIdx.y is the head, the block's warps (halves) take tokens in turn.
+template <int NG> struct Kv4Lanes {
+  static constexpr int W = 8 * NG;                        // words of codes of a head
+  static constexpr int ITEMS = NG <= 2 ? 1 : 2;           // words of a lane
+  static constexpr int LANES = NG == 1 ? 16 : 32;
+  static constexpr int STEP = 256 / LANES;                // tokens that a block has at a time
+  static __device__ __forceinline__ bool is_value(int lane, int item) { return ITEMS == 2 ? item == 1 : lane >= W; }
+  static __device__ __forceinline__ int word(int lane) { return ITEMS == 2 ? lane : lane % W; }
+};
+
+// Adding it rounds a float below 2^22 to a whole number, ties to even, and leaves that number in the low bits.
+constexpr float kRoundMagic = 12582912.0f;      // 1.5 * 2^23
+// rint(x / s) for |x / s| < 16, x / s as the correctly rounded quotient: Markstein's method (1990), which takes the correctly rounded reciprocal, a
+// quotient by it, the remainder by one fma (exact) and a second fma that corrects the quotient. (Ties of bfloat16 numbers are common: a
+// quotient that is only near would send most warps through a division.)
+// The whole number comes plus `add` (which is whole, too).
+__device__ __forceinline__ float kv4_quotient(float x, float s, float reciprocal, float add) {
+  const float q = x * reciprocal;
+  return __fadd_rn(__fadd_rn(fmaf(fmaf(-q, s, x), reciprocal, q), kRoundMagic), add - kRoundMagic);
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float d;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+// ROUNDS: tokens that a thread takes one after the other, and works out its place in a head for once.
+template <typename T, int NG, int ROUNDS>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const T* __restrict__ k, const T* __restrict__ v, long long k_stride, long long v_stride,
-                                                         const int* __restrict__ slots, Kv4Planes c, long long units, int vec, int* status) {
+                                                         const int* __restrict__ slots, Kv4Planes c, int tokens, int vec, int* status) {
   pdl_sync();
-  constexpr int W = 8 * NG;                        // words of codes of a head
-  constexpr int ITEMS = NG <= 2 ? 1 : 2;           // of a lane
-  constexpr int LANES = NG == 1 ? 16 : 32;
-  const int lane = threadIdx.x & (LANES - 1);
-  const long long unit = static_cast<long long>(blockIdx.x) * (256 / LANES) + threadIdx.x / LANES;
-  const bool there = unit < units;
-  const long long token = there ? unit / c.kv_heads : 0;
-  const int head = there ? static_cast<int>(unit % c.kv_heads) : 0;
-  const int slot = there ? slots[token] : -1;
-  const bool writes = slot >= 0 && static_cast<unsigned int>(slot) < c.slots;
-  if (slot >= 0 && !writes && lane == 0) *reinterpret_cast<volatile int*>(status) = kStatusBadSlot;
-  float x[ITEMS][8];
-  bool fine = true;
-#pragma unroll
-  for (int i = 0; i < ITEMS; ++i) {
-    const bool is_v = ITEMS == 2 ? i == 1 : lane >= W;
-    const int word = ITEMS == 2 ? lane : lane % W;
-    const T* row = is_v ? v + token * v_stride : k + token * k_stride;
-    const int dims = writes && word < W ? c.head_dim - word * 8 : 0;
-    load8(row + static_cast<long long>(head) * c.head_dim + word * 8, dims, vec != 0, x[i]);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) fine = fine && fabsf(x[i][e]) < kKv4Limit;
-  }
-  const uint32_t all = __ballot_sync(0xffffffffu, fine);
+  using L = Kv4Lanes<NG>;
+  const int lane = threadIdx.x & (L::LANES - 1), head = blockIdx.y, word = L::word(lane);
   const uint32_t mine = NG == 1 ? 0xffffu << (threadIdx.x & 16) : 0xffffffffu;
-  fine = (all & mine) == mine;
-  const long long at = kv4_row(writes ? slot : 0, head, c.kv_heads, c.page_size);
+  const int dims = word < L::W ? c.head_dim - word * 8 : 0;
+  const T* src[L::ITEMS];
+  long long stride[L::ITEMS];
 #pragma unroll
-  for (int i = 0; i < ITEMS; ++i) {
-    const bool is_v = ITEMS == 2 ? i == 1 : lane >= W;
-    const int word = ITEMS == 2 ? lane : lane % W;
-    float lo = 0.0f, hi = 0.0f;
+  for (int i = 0; i < L::ITEMS; ++i) {
+    src[i] = (L::is_value(lane, i) ? v : k) + static_cast<long long>(head) * c.head_dim + word * 8;
+    stride[i] = L::is_value(lane, i) ? v_stride : k_stride;
+  }
+#pragma unroll 2
+  for (int round = 0; round < ROUNDS; ++round) {
+    const int token = blockIdx.x * (ROUNDS * L::STEP) + round * L::STEP + threadIdx.x / L::LANES;
+    const int slot = token < tokens ? slots[token] : -1;
+    const bool writes = slot >= 0 && static_cast<unsigned int>(slot) < c.slots;
+    if (slot >= 0 && !writes && lane == 0) *reinterpret_cast<volatile int*>(status) = kStatusBadSlot;
+    float x[L::ITEMS][8], lo[L::ITEMS], hi[L::ITEMS];
+    bool fine = true;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) lo = fminf(lo, x[i][e]), hi = fmaxf(hi, x[i][e]);
+    for (int i = 0; i < L::ITEMS; ++i) {
+      load8(src[i] + token * stride[i], writes ? dims : 0, vec != 0, x[i]);
+      lo[i] = hi[i] = 0.0f;
 #pragma unroll
-    for (int o = 1; o <= 2; o <<= 1) {
-      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+      for (int e = 0; e < 8; ++e) lo[i] = min_nan(lo[i], x[i][e]), hi[i] = max_nan(hi[i], x[i][e]);
+      fine = fine && hi[i] < kKv4Limit && lo[i] > -kKv4Limit;      // (false for NaN)
     }
-    uint32_t codes = 0, w = is_v ? 0u : kKv4NaN;
-    if (fine) {
-      const float s = kv4_step(lo, hi);
-      const float z = rintf(__fdiv_rn(-lo, s));
+    fine = (__ballot_sync(0xffffffffu, fine) & mine) == mine;
+    const int at = kv4_row(writes ? slot : 0, head, c);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float q = fminf(fmaxf(rintf(__fdiv_rn(x[i][e], s)) + z, 0.0f), 15.0f);
-        codes |= static_cast<uint32_t>(q) << (4 * e);
+    for (int i = 0; i < L::ITEMS; ++i) {
+      const bool is_v = L::is_value(lane, i);
+#pragma unroll
+      for (int o = 1; o <= 2; o <<= 1) {
+        lo[i] = fminf(lo[i], __shfl_xor_sync(0xffffffffu, lo[i], o));
+        hi[i] = fmaxf(hi[i], __shfl_xor_sync(0xffffffffu, hi[i], o));
       }
-      w = (__float_as_uint(s) >> 16) | static_cast<uint32_t>(z);
-    }
-    if (writes && word < W) {
-      (is_v ? c.v_codes : c.k_codes)[at * W + word] = codes;
-      if ((word & 3) == 0) (is_v ? c.v_words : c.k_words)[at * (W / 4) + word / 4] = static_cast<uint16_t>(w);
+      uint32_t codes = 0, w = is_v ? 0u : kKv4NaN;
+      if (fine) {
+        const float s = kv4_step(lo[i], hi[i]), reciprocal = __frcp_rn(s);
+        const float z = kv4_quotient(-lo[i], s, reciprocal, 0.0f);
+        // four codes as the digits of one number, whose bits 2^23 shows. (rint(x / s) >= rint(lo / s) = -z: only the upper end is to be clamped)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float four = 0.0f;
+#pragma unroll
+          for (int e = 3; e >= 0; --e) four = fmaf(four, 16.0f, fminf(kv4_quotient(x[i][4 * h + e], s, reciprocal, z), 15.0f));
+          codes |= (__float_as_uint(four + 8388608.0f) & 0xffffu) << (16 * h);
+        }
+        w = (__float_as_uint(s) >> 16) | (__float_as_uint(z + 8388608.0f) & 15u);
+      }
+      if (writes && word < L::W) {
+        (is_v ? c.v_codes : c.k_codes)[static_cast<long long>(at) * L::W + word] = codes;
+        if ((word & 3) == 0) (is_v ? c.v_words : c.k_words)[static_cast<long long>(at) * (L::W / 4) + word / 4] = static_cast<uint16_t>(w);
+      }
     }
   }
 }
 
-// A thread: eight dimensions of a row of keys or of values.
-template <typename T>
+template <typename T, int NG, int ROUNDS>
 __global__ void __launch_bounds__(256) kv4_read_kernel(Kv4Planes c, const int* __restrict__ slots, T* __restrict__ k, T* __restrict__ v, long long k_stride,
-                                                       long long v_stride, int words, long long items, int vec, int* status) {
+                                                       long long v_stride, int tokens, int vec, int* status) {
   pdl_sync();
-  const long long id = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
-  if (id >= items) return;
-  const int word = static_cast<int>(id % words);
-  const long long rest = id / words;
-  const bool is_v = rest & 1;
-  const long long unit = rest >> 1, token = unit / c.kv_heads;
-  const int head = static_cast<int>(unit % c.kv_heads);
-  const int slot = slots[token];
-  if (slot < 0) return;
-  if (static_cast<unsigned int>(slot) >= c.slots) {
-    *reinterpret_cast<volatile int*>(status) = kStatusBadSlot;
-    return;
-  }
-  const int left = c.head_dim - word * 8;
-  if (left <= 0) return;
-  const long long at = kv4_row(slot, head, c.kv_heads, c.page_size);
-  const uint32_t codes = (is_v ? c.v_codes : c.k_codes)[at * words + word];
-  const uint32_t w = (is_v ? c.v_words : c.k_words)[at * (words / 4) + word / 4];
-  const float s = __uint_as_float((w & 0xffe0u) << 16);
-  const int z = w & 15;
-  float x[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = s * static_cast<float>(static_cast<int>((codes >> (4 * e)) & 15) - z);
-  T* dst = (is_v ? v + token * v_stride : k + token * k_stride) + static_cast<long long>(head) * c.head_dim + word * 8;
-  if (vec && left >= 8) {
-    constexpr int N = Vec16<T>::N;
-#pragma unroll
-    for (int i = 0; i < 8; i += N) {
-      Vec16<T> t;
-#pragma unroll
-      for (int e = 0; e < N; ++e) t.v[e] = x[i + e];
-      t.store(dst + i);
+  using L = Kv4Lanes<NG>;
+  const int lane = threadIdx.x & (L::LANES - 1), head = blockIdx.y, word = L::word(lane), left = c.head_dim - word * 8;
+  if (word >= L::W || left <= 0) return;
+#pragma unroll 4
+  for (int round = 0; round < ROUNDS; ++round) {
+    const int token = blockIdx.x * (ROUNDS * L::STEP) + round * L::STEP + threadIdx.x / L::LANES;
+    const int slot = token < tokens ? slots[token] : -1;
+    if (slot < 0) continue;
+    if (static_cast<unsigned int>(slot) >= c.slots) {
+      if (lane == 0) *reinterpret_cast<volatile int*>(status) = kStatusBadSlot;
+      continue;
     }
-  } else {
+    const int at = kv4_row(slot, head, c);
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (e < left) st(dst + e, x[e]);
+    for (int i = 0; i < L::ITEMS; ++i) {
+      const bool is_v = L::is_value(lane, i);
+      const uint32_t codes = (is_v ? c.v_codes : c.k_codes)[static_cast<long long>(at) * L::W + word];
+      const uint32_t w = (is_v ? c.v_words : c.k_words)[static_cast<long long>(at) * (L::W / 4) + word / 4];
+      const float s = __uint_as_float((w & 0xffe0u) << 16);
+      const float z = __uint_as_float((w & 15u) | 0x4b000000u);          // 2^23 + z, and 2^23 + code: their difference is exact
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = s * (__uint_as_float(((codes >> (4 * e)) & 15u) | 0x4b000000u) - z);
+      T* dst = (is_v ? v + token * v_stride : k + token * k_stride) + static_cast<long long>(head) * c.head_dim + word * 8;
+      if (vec && left >= 8) {
+        constexpr int N = Vec16<T>::N;
+#pragma unroll
+        for (int j = 0; j < 8; j += N) {
+          Vec16<T> t;
+#pragma unroll
+          for (int e = 0; e < N; ++e) t.v[e] = x[j + e];
+          t.store(dst + j);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (e < left) st(dst + e, x[e]);
+      }
+    }
   }
 }
 
@@ -133,35 +169,52 @@ static bool kv4_rows_aligned(const void* k, const void* v, long long k_stride, l
          head_dim * size % 16 == 0;
 }
 
-template <typename T>
-static void launch_kv4_append(const T* k, const T* v, long long k_stride, long long v_stride, const int* slots, const Kv4Planes& c, int tokens, cudaStream_t s) {
-  const long long units = static_cast<long long>(tokens) * c.kv_heads;
+template <typename T, int NG, int ROUNDS>
+static void launch_kv4(bool append, T* k, T* v, long long k_stride, long long v_stride, const int* slots, const Kv4Planes& c, int tokens, cudaStream_t s) {
   const int vec = kv4_rows_aligned(k, v, k_stride, v_stride, c.head_dim, sizeof(T)) ? 1 : 0;
-  const int ng = (c.head_dim + 63) / 64;
-  const int blocks = ceil_div(units, ng == 1 ? 16 : 8);
-  switch (ng) {
-    case 1: TIE_LAUNCH((kv4_append_kernel<T, 1>), blocks, 256, 0, s, k, v, k_stride, v_stride, slots, c, units, vec, status_word()); break;
-    case 2: TIE_LAUNCH((kv4_append_kernel<T, 2>), blocks, 256, 0, s, k, v, k_stride, v_stride, slots, c, units, vec, status_word()); break;
-    case 3: TIE_LAUNCH((kv4_append_kernel<T, 3>), blocks, 256, 0, s, k, v, k_stride, v_stride, slots, c, units, vec, status_word()); break;
-    default: TIE_LAUNCH((kv4_append_kernel<T, 4>), blocks, 256, 0, s, k, v, k_stride, v_stride, slots, c, units, vec, status_word()); break;
+  const dim3 grid(ceil_div(tokens, ROUNDS * Kv4Lanes<NG>::STEP), c.kv_heads);
+  if (append) TIE_LAUNCH((kv4_append_kernel<T, NG, ROUNDS>), grid, 256, 0, s, k, v, k_stride, v_stride, slots, c, tokens, vec, status_word());
+  else TIE_LAUNCH((kv4_read_kernel<T, NG, ROUNDS>), grid, 256, 0, s, c, slots, k, v, k_stride, v_stride, tokens, vec, status_word());
+}
+
+// Four tokens a thread where that still leaves every SM eight blocks: 8,192 tokens of 8 heads of 128 in and out 28 us against 30 with one; but
+// 2,049 of 5 heads of 96 11.1 against 8.8, eight tokens 4.8 against 3.3.
+template <typename T, int NG>
+static void launch_kv4(bool append, T* k, T* v, long long k_stride, long long v_stride, const int* slots, const Kv4Planes& c, int tokens, cudaStream_t s) {
+  if (static_cast<long long>(tokens / (4 * Kv4Lanes<NG>::STEP)) * c.kv_heads >= 148 * 8) launch_kv4<T, NG, 4>(append, k, v, k_stride, v_stride, slots, c, tokens, s);
+  else launch_kv4<T, NG, 1>(append, k, v, k_stride, v_stride, slots, c, tokens, s);
+}
+
+template <typename T>
+static void launch_kv4(bool append, void* k, void* v, long long k_stride, long long v_stride, const int* slots, const Kv4Planes& c, int tokens, cudaStream_t s) {
+  T *kt = static_cast<T*>(k), *vt = static_cast<T*>(v);
+  switch ((c.head_dim + 63) / 64) {
+    case 1: launch_kv4<T, 1>(append, kt, vt, k_stride, v_stride, slots, c, tokens, s); break;
+    case 2: launch_kv4<T, 2>(append, kt, vt, k_stride, v_stride, slots, c, tokens, s); break;
+    case 3: launch_kv4<T, 3>(append, kt, vt, k_stride, v_stride, slots, c, tokens, s); break;
+    default: launch_kv4<T, 4>(append, kt, vt, k_stride, v_stride, slots, c, tokens, s); break;
   }
 }
 
-template <typename T>
-static void launch_kv4_read(T* k, T* v, long long k_stride, long long v_stride, const int* slots, const Kv4Planes& c, int tokens, cudaStream_t s) {
-  const int words = (c.head_dim + 63) / 64 * 8;
-  const long long items = static_cast<long long>(tokens) * c.kv_heads * 2 * words;
-  const int vec = kv4_rows_aligned(k, v, k_stride, v_stride, c.head_dim, sizeof(T)) ? 1 : 0;
-  TIE_LAUNCH(kv4_read_kernel<T>, ceil_div(items, 256), 256, 0, s, c, slots, k, v, k_stride, v_stride, words, items, vec, status_word());
+static Kv4Planes kv4_planes(const void* k_codes, const void* k_words, const void* v_codes, const void* v_words, int kv_heads, int head_dim, int page_size, long long pages) {
+  int shift = 0;
+  while (shift < 30 && (1 << shift) < page_size) ++shift;
+  return {static_cast<uint32_t*>(const_cast<void*>(k_codes)), static_cast<uint32_t*>(const_cast<void*>(v_codes)), static_cast<uint16_t*>(const_cast<void*>(k_words)),
+          static_cast<uint16_t*>(const_cast<void*>(v_words)), kv_heads, page_size, (1 << shift) == page_size ? shift : -1, head_dim,
+          static_cast<unsigned int>(pages * page_size)};
 }
 
-static int kv4_check(const char* name, const Kv4Planes& c, int tokens, long long pages) {
-  TIE_REQUIRE(tokens >= 0 && c.kv_heads > 0 && c.page_size > 0 && c.head_dim > 0 && c.head_dim <= 256, "%s: bad sizes (tokens %d, kv heads %d, page size %d, head size %d)",
-              name, tokens, c.kv_heads, c.page_size, c.head_dim);
+static int launch_kv4(const char* name, bool append, int dtype, const Kv4Planes& c, void* k, void* v, long long k_stride, long long v_stride, const int* slots, int tokens,
+                      long long pages, cudaStream_t s) {
+  TIE_REQUIRE(tokens >= 0 && c.kv_heads > 0 && c.kv_heads <= 65535 && c.page_size > 0 && c.head_dim > 0 && c.head_dim <= 256,
+              "%s: bad sizes (tokens %d, kv heads %d, page size %d, head size %d)", name, tokens, c.kv_heads, c.page_size, c.head_dim);
   TIE_REQUIRE(pages > 0 && pages * c.page_size < (1LL << 31), "%s: %lld pages of %d tokens: slots are 32-bit numbers", name, pages, c.page_size);
-  TIE_REQUIRE(static_cast<long long>(tokens) * c.kv_heads * 64 < (1LL << 31) * 256, "%s: too many rows", name);
+  TIE_REQUIRE(pages * c.page_size * c.kv_heads < (1LL << 31), "%s: planes of %lld x %d x %d rows: rows are 32-bit numbers", name, pages, c.kv_heads, c.page_size);
   TIE_REQUIRE(status_word() != nullptr, "%s: cannot allocate the status word", name);
-  return kOk;
+  if (tokens == 0) return kOk;
+  if (dtype == TIE_F32) launch_kv4<float>(append, k, v, k_stride, v_stride, slots, c, tokens, s);
+  else launch_kv4<__nv_bfloat16>(append, k, v, k_stride, v_stride, slots, c, tokens, s);
+  TIE_RETURN_LAUNCH(name);
 }
 
 }  // namespace tie
@@ -171,24 +224,13 @@ using namespace tie;
 // k, v [tokens, kv_heads * head_dim] (rows strides apart) into the planes at slots[t]; a slot below zero writes nothing.
 TIE_API int tie_kv4_append(int dtype, const void* k, const void* v, long long k_stride, long long v_stride, const int* slots, void* k_codes, void* k_words,
                            void* v_codes, void* v_words, int tokens, int kv_heads, int head_dim, int page_size, long long pages, cudaStream_t s) {
-  const Kv4Planes c{static_cast<uint32_t*>(k_codes), static_cast<uint32_t*>(v_codes), static_cast<uint16_t*>(k_words), static_cast<uint16_t*>(v_words),
-                    kv_heads, page_size, head_dim, static_cast<unsigned int>(pages * page_size)};
-  if (const int bad = kv4_check("kv4_append", c, tokens, pages)) return bad;
-  if (tokens == 0) return kOk;
-  if (dtype == TIE_F32) launch_kv4_append(static_cast<const float*>(k), static_cast<const float*>(v), k_stride, v_stride, slots, c, tokens, s);
-  else launch_kv4_append(static_cast<const __nv_bfloat16*>(k), static_cast<const __nv_bfloat16*>(v), k_stride, v_stride, slots, c, tokens, s);
-  TIE_RETURN_LAUNCH("kv4_append");
+  return launch_kv4("kv4_append", true, dtype, kv4_planes(k_codes, k_words, v_codes, v_words, kv_heads, head_dim, page_size, pages), const_cast<void*>(k),
+                    const_cast<void*>(v), k_stride, v_stride, slots, tokens, pages, s);
 }
 
 // The values at slots[t] into k, v [tokens, kv_heads * head_dim]; rows whose slot is below zero are left as they are.
 TIE_API int tie_kv4_read(int dtype, const void* k_codes, const void* k_words, const void* v_codes, const void* v_words, const int* slots, void* k, void* v,
                          long long k_stride, long long v_stride, int tokens, int kv_heads, int head_dim, int page_size, long long pages, cudaStream_t s) {
-  const Kv4Planes c{static_cast<uint32_t*>(const_cast<void*>(k_codes)), static_cast<uint32_t*>(const_cast<void*>(v_codes)),
-                    static_cast<uint16_t*>(const_cast<void*>(k_words)), static_cast<uint16_t*>(const_cast<void*>(v_words)),
-                    kv_heads, page_size, head_dim, static_cast<unsigned int>(pages * page_size)};
-  if (const int bad = kv4_check("kv4_read", c, tokens, pages)) return bad;
-  if (tokens == 0) return kOk;
-  if (dtype == TIE_F32) launch_kv4_read(static_cast<float*>(k), static_cast<float*>(v), k_stride, v_stride, slots, c, tokens, s);
-  else launch_kv4_read(static_cast<__nv_bfloat16*>(k), static_cast<__nv_bfloat16*>(v), k_stride, v_stride, slots, c, tokens, s);
-  TIE_RETURN_LAUNCH("kv4_read");
+  return launch_kv4("kv4_read", false, dtype, kv4_planes(k_codes, k_words, v_codes, v_words, kv_heads, head_dim, page_size, pages), k, v, k_stride, v_stride, slots,
+                    tokens, pages, s);
 }

@@ -101,7 +101,7 @@ def _int32(what: str, name: str, t, n: int) -> None:
 
 def kv4_cache(pages: int, kv_heads: int, page_size: int, head_dim: int, device="cuda") -> Kv4Cache:
     """An empty cache for one layer (of any number of requests)."""
-    _need(pages > 0 and kv_heads > 0 and page_size > 0 and 0 < head_dim <= 256 and pages * page_size < 2 ** 31,
+    _need(pages > 0 and kv_heads > 0 and page_size > 0 and 0 < head_dim <= 256 and pages * kv_heads * page_size < 2 ** 31,
           f"kv4_cache: bad sizes (pages {pages}, kv heads {kv_heads}, page size {page_size}, head size {head_dim}, at most 256)")
     padded = -(-head_dim // 64) * 64
 
@@ -124,8 +124,8 @@ def _check_cache(what: str, c: Kv4Cache) -> tuple:
     if width != 16 * words or not (kc.dtype is vc.dtype is torch.uint8 and kw.dtype is vw.dtype is torch.int16) or kw.numel() != n or vw.numel() != n or \
             vc.numel() != 16 * n or not (kc.is_contiguous() and kw.is_contiguous() and vc.is_contiguous() and vw.is_contiguous()):
         _fail(f"{what}: planes must be contiguous, codes uint8 [pages, kv_heads, page_size, {16 * words}] and words int16 [..., {words}]")
-    if n == 0 or pages * size >= 2 ** 31:
-        _fail(f"{what}: slots must be 32-bit numbers, of one page at least")
+    if n == 0 or pages * heads * size >= 2 ** 31:
+        _fail(f"{what}: planes must have one row at least and less than 2^31 (pages x kv heads x page size)")
     planes = kc.data_ptr(), kw.data_ptr(), vc.data_ptr(), vw.data_ptr()
     if (planes[0] | planes[1] | planes[2] | planes[3]) & 15:
         _fail(f"{what}: planes must be 16-byte aligned")
