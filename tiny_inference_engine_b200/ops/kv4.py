@@ -85,18 +85,15 @@ _I32 = torch.int32
 
 def _stream(what: str, *ts) -> int:
     """The current stream, once every tensor is known to be on the current device."""
-    here = torch._C._cuda_getDevice() if ts[0].is_cuda else -1
+    here = _CURRENT_DEVICE() if ts[0].is_cuda else -1
     for t in ts:
         if t.get_device() != here or here < 0:
             _fail("kernel arguments must be CUDA tensors: the engine has no CPU path" if not t.is_cuda else
                   f"{what}: all tensors must be on the current device, {here}, got one on {t.device}")
-    return torch._C._cuda_getCurrentRawStream(here)
+    return _RAW_STREAM(here)
 
 
-def _int32(what: str, name: str, t, n: int) -> None:
-    """A contiguous vector of n int32 numbers."""
-    if t.dtype is not _I32 or t.numel() != n or not t.is_contiguous():
-        _fail(f"{what}: {name} must be contiguous int32 [{n}]")
+_CURRENT_DEVICE, _RAW_STREAM = getattr(torch._C, "_cuda_getDevice", None), getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def kv4_cache(pages: int, kv_heads: int, page_size: int, head_dim: int, device="cuda") -> Kv4Cache:
@@ -143,7 +140,8 @@ def _check_rows(what: str, c: Kv4Cache, k, v, slots) -> tuple:
     (k_stride, k_step), (v_stride, v_step) = k.stride(), v.stride()
     if (k_step != 1 or v_step != 1) and width > 1:
         _fail(f"{what}: k and v must be [T, {width}] with contiguous rows")
-    _int32(what, "slots", slots, shape[0])
+    if slots.dtype is not _I32 or slots.numel() != shape[0] or not slots.is_contiguous():
+        _fail(f"{what}: slots must be contiguous int32 [{shape[0]}]")
     return dtype, planes, sizes, shape[0], k_stride, v_stride, _stream(what, k, v, slots, c[0], c[1], c[2], c[3])
 
 
@@ -197,10 +195,9 @@ def _check_attention(what, q, cache, out, query_start, context_lens, block_table
     if len(out_shape) != 2 or out_shape[0] != shape[0] or out_shape[1] != width or not out.is_contiguous():
         _fail(f"{what}: out must be contiguous [T, {width}]")
     S = context_lens.numel()
-    _int32(what, "query_start", query_start, S + 1)
-    _int32(what, "context_lens", context_lens, S)
-    if len(table_shape) != 2 or table_shape[0] != S or block_tables.dtype is not _I32 or not block_tables.is_contiguous():
-        _fail(f"{what}: block_tables must be contiguous int32 [{S}, pages]")
+    if not (query_start.dtype is context_lens.dtype is block_tables.dtype is _I32) or query_start.numel() != S + 1 or len(table_shape) != 2 or \
+            table_shape[0] != S or not (query_start.is_contiguous() and context_lens.is_contiguous() and block_tables.is_contiguous()):
+        _fail(f"{what}: query_start [{S + 1}], context_lens [{S}] and block_tables [{S}, pages] must be contiguous int32")
     if not 0 <= n <= 65535 or (seq_list is None and n > S):
         _fail(f"{what}: {n} of {S} sequences (at most 65,535 a call)")
     if not 0 <= window < 2 ** 30:
@@ -273,12 +270,9 @@ def step_arrays(n: int, rows: int, columns: int, device="cuda") -> StepArrays:
 def _check_tables(what, requests, lens, tables, free_pages, free_count, page_size) -> tuple:
     """(sequences, requests of the state, columns of its tables, pages)"""
     shape, n, held, pages = tables.shape, requests.numel(), lens.numel(), free_pages.numel()
-    _int32(what, "requests", requests, n)
-    _int32(what, "lens", lens, held)
-    _int32(what, "free_pages", free_pages, pages)
-    _int32(what, "free_count", free_count, 1)
-    if len(shape) != 2 or shape[0] != held or tables.dtype is not _I32 or not tables.is_contiguous():
-        _fail(f"{what}: tables must be contiguous int32 [{held}, pages]")
+    if not (requests.dtype is lens.dtype is free_pages.dtype is free_count.dtype is tables.dtype is _I32) or free_count.numel() != 1 or len(shape) != 2 or \
+            shape[0] != held or not (requests.is_contiguous() and lens.is_contiguous() and free_pages.is_contiguous() and tables.is_contiguous()):
+        _fail(f"{what}: requests, lens [{held}], tables [{held}, pages], free_pages and free_count [1] must be contiguous int32")
     if page_size <= 0:
         _fail(f"{what}: page size must be positive")
     return n, held, shape[1], pages
@@ -300,16 +294,14 @@ def step_tables(requests, counts, lens, tables, free_pages, free_count, page_siz
     n, held, width, pages = _check_tables(what, requests, lens, tables, free_pages, free_count, page_size)
     query_start, context_lens, positions, seq_of_row, slots, block_tables, free_left, status = arrays
     rows, shape = slots.numel(), block_tables.shape
-    _int32(what, "counts", counts, n)
-    _int32(what, "arrays.query_start", query_start, n + 1)
-    _int32(what, "arrays.context_lens", context_lens, n)
-    _int32(what, "arrays.positions", positions, rows)
-    _int32(what, "arrays.seq_of_row", seq_of_row, rows)
-    _int32(what, "arrays.slots", slots, rows)
-    _int32(what, "arrays.free_left", free_left, 1)
-    _int32(what, "arrays.status", status, 1)
-    if len(shape) != 2 or shape[0] != n or block_tables.dtype is not _I32 or not block_tables.is_contiguous() or not 0 < shape[1] <= width:
-        _fail(f"{what}: arrays.block_tables must be contiguous int32 [{n}, up to {width}]")
+    if not (counts.dtype is query_start.dtype is context_lens.dtype is positions.dtype is seq_of_row.dtype is slots.dtype is block_tables.dtype is
+            free_left.dtype is status.dtype is _I32) or counts.numel() != n or query_start.numel() != n + 1 or context_lens.numel() != n or \
+            positions.numel() != rows or seq_of_row.numel() != rows or free_left.numel() != 1 or status.numel() != 1 or not (
+            counts.is_contiguous() and query_start.is_contiguous() and context_lens.is_contiguous() and positions.is_contiguous() and
+            seq_of_row.is_contiguous() and slots.is_contiguous()):
+        _fail(f"{what}: counts [{n}] and arrays (step_arrays makes them for {n} sequences) must be contiguous int32")
+    if len(shape) != 2 or shape[0] != n or not block_tables.is_contiguous() or not 0 < shape[1] <= width:
+        _fail(f"{what}: arrays.block_tables must be contiguous [{n}, up to {width}]")
     stream = _stream(what, requests, counts, lens, tables, free_pages, free_count, query_start, context_lens, positions, seq_of_row, slots, block_tables,
                      free_left, status)
     call("tie_step_tables", requests.data_ptr(), counts.data_ptr(), lens.data_ptr(), tables.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(),
@@ -323,7 +315,8 @@ def release_tables(requests, lens, tables, free_pages, free_count, page_size: in
     (int32 [1], else 0), where a request or length cannot be or the stack would overflow."""
     what = "release_tables"
     n, held, width, pages = _check_tables(what, requests, lens, tables, free_pages, free_count, page_size)
-    _int32(what, "status", status, 1)
+    if status.dtype is not _I32 or status.numel() != 1:
+        _fail(f"{what}: status must be int32 [1]")
     stream = _stream(what, requests, lens, tables, free_pages, free_count, status)
     call("tie_release_tables", requests.data_ptr(), lens.data_ptr(), tables.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(), status.data_ptr(), n,
          held, width, pages, page_size, stream)
