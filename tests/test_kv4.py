@@ -105,3 +105,35 @@ def test_step_tables_refuse():
     refused(ops.release_tables, **good, status=i32(0, 0))
     for bad in ((-1, 1, 1), (1, -1, 1), (1, 1, 0)):
         refused(ops.step_arrays, *bad, device="cpu")
+
+
+def test_cache_manager_counts_the_bytes_of_4_bits():
+    from tiny_inference_engine_b200.cache import CacheManager
+    from tiny_inference_engine_b200.errors import UnsupportedError
+    from tiny_inference_engine_b200.parts.base import CacheNeed
+    needs = [CacheNeed("full", 8, 128)] * 3 + [CacheNeed("window", 2, 96, 64)]
+    wide = CacheManager(needs, 16, num_pages=5, dtype=torch.bfloat16)
+    four = CacheManager(needs, 16, num_pages=5, dtype=torch.bfloat16, kv_bits=4)
+    assert wide.bytes_per_page == 16 * 2 * 2 * (3 * 8 * 128 + 2 * 96)
+    assert four.bytes_per_page == 16 * 2 * (3 * 8 * 72 + 2 * 72)              # 64 bytes of codes and 8 of words; 96 is padded to 128
+    made = CacheManager(needs, 16, num_pages=5, dtype=torch.bfloat16, device="cpu", kv_bits=4)
+    assert sum(t.numel() * t.element_size() for pair in made.storage for t in pair) == 5 * four.bytes_per_page
+    view = made.layer_cache(2, True)
+    assert view.k is None and view.kv4.head_dim == 128 and tuple(view.kv4.k_codes.shape) == (5, 8, 16, 64) and tuple(view.kv4.v_words.shape) == (5, 8, 16, 4)
+    view.kv4.v_codes.fill_(7)                          # the planes are apart
+    assert int((made.storage[0][0] == 7).sum()) == view.kv4.v_codes.numel() and int(made.layer_cache(2, True).kv4.k_codes.sum()) == 0
+    for need in (CacheNeed("full", 1, 64, value_dim=-1), CacheNeed("full", 1, 64, value_dim=32), CacheNeed("full", 1, 512), CacheNeed("window", 1, 64, 8, keep_first=4)):
+        with pytest.raises(UnsupportedError):
+            CacheManager([need], 16, num_pages=5, kv_bits=4)
+    refused(CacheManager, needs, 16, num_pages=5, kv_bits=8, match="kv_bits")
+
+
+def test_designs_whose_mixers_know_no_4_bits_are_refused():
+    import plain_misudra
+    from tiny_inference_engine_b200 import make_cache
+    from tiny_inference_engine_b200.config import misudra_spec, parse_misudra_config
+    from tiny_inference_engine_b200.errors import UnsupportedError
+    from tiny_inference_engine_b200.parts.model import Model
+    cfg = plain_misudra.make_config([plain_misudra.latent_layer(mlp=plain_misudra.dense())])
+    with pytest.raises(UnsupportedError, match="4 bits"):
+        make_cache(Model(misudra_spec(parse_misudra_config(cfg)), torch.float32), num_pages=4, device="cpu", kv_bits=4)

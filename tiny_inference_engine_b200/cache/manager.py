@@ -33,7 +33,7 @@ from dataclasses import dataclass, field
 
 import numpy as np
 
-from ..errors import CapacityError, InvalidArgument
+from ..errors import CapacityError, InvalidArgument, UnsupportedError
 from .block_pool import BlockPool
 
 FREED = -1
@@ -99,14 +99,18 @@ class CacheManager:
 
     def __init__(self, needs, page_size: int, num_pages: int | None = None, budget_bytes: int | None = None,
                  dtype=None, device=None, state_slots=None, window_requests: int | None = None,
-                 window_step_tokens: int = 0):
+                 window_step_tokens: int = 0, kv_bits: int = 0):
         """`num_pages` (or what `budget_bytes` buys) is the page count of the groups that keep every key.
         With `window_requests` a window group holds only what that many requests can use at once:
-        the pages of `window + window_step_tokens` tokens, and two more for the edges, per request."""
+        the pages of `window + window_step_tokens` tokens, and two more for the edges, per request.
+        `kv_bits` 4: keys and values in 4 bits (ops/kv4.py), 4.5 bits a value with their scales, whatever `dtype` is; 0: in `dtype`."""
         if page_size <= 0:
             raise InvalidArgument(f"page size must be positive, got {page_size}")
+        if kv_bits not in (0, 4):
+            raise InvalidArgument(f"kv_bits must be 4, or 0 for the compute type, got {kv_bits}")
         self.page_size = page_size
         self.dtype = dtype
+        self.kv_bits = kv_bits
         keyed: dict[tuple, list[int]] = {}
         for i, need in enumerate(needs):
             if need is None:
@@ -122,8 +126,10 @@ class CacheManager:
         self._kept_pages = [blocks_for(g.keep_first, page_size) for g in self.groups]
         self._entry_group = {e: gi for gi, g in enumerate(self.groups) for e in g.entries}
         self._entry_plane = {e: pi for g in self.groups for pi, e in enumerate(g.entries)}
+        if kv_bits and any(g.value_dim or g.keep_first or g.head_dim > 256 for g in self.groups):
+            raise UnsupportedError("a cache in 4 bits holds keys and values of one size up to 256, and windows without kept first tokens")
         elem = 4 if dtype is None else _elem_size(dtype)
-        group_bytes = [len(g.entries) * g.kv_heads * page_size * _row_elems(g) * elem for g in self.groups]
+        group_bytes = [len(g.entries) * g.kv_heads * page_size * (2 * _kv4_row_bytes(g.head_dim) if kv_bits else _row_elems(g) * elem) for g in self.groups]
         # what a window group can ever use (None: as many pages as the other groups)
         bounded = [None] * len(self.groups)
         if window_requests is not None:
@@ -153,7 +159,11 @@ class CacheManager:
         if device is not None:
             import torch
             for g, n in zip(self.groups, self.group_pages):
-                if g.value_dim == VALUES_IN_KEYS:
+                if kv_bits:          # codes and words of every plane's keys and values (zeros stand for zeros)
+                    shape = (len(g.entries), 2, n, g.kv_heads, page_size)
+                    self.storage.append((torch.zeros((*shape, _kv4_row_bytes(g.head_dim) // 9 * 8), dtype=torch.uint8, device=device),
+                                         torch.zeros((*shape, _kv4_row_bytes(g.head_dim) // 18), dtype=torch.int16, device=device)))
+                elif g.value_dim == VALUES_IN_KEYS:
                     self.storage.append(torch.zeros((len(g.entries), 1, n, g.kv_heads, page_size, g.head_dim),
                                                     dtype=dtype, device=device))
                 elif g.value_dim:    # keys of every plane, then values of every plane, in one flat buffer
@@ -310,6 +320,10 @@ class CacheManager:
         gi, pi = self._entry_group[entry], self._entry_plane[entry]
         st = self.storage[gi]
         g = self.groups[gi]
+        if self.kv_bits:
+            from ..ops import Kv4Cache
+            codes, words = st[0][pi], st[1][pi]
+            return LayerCache(None, None, gi, writes, Kv4Cache(codes[0], words[0], codes[1], words[1], g.head_dim))
         if g.value_dim == VALUES_IN_KEYS:
             return LayerCache(st[pi, 0], st[pi, 0], gi, writes)
         if g.value_dim:
@@ -332,6 +346,11 @@ def _row_elems(g: GroupSpec) -> int:
     if g.value_dim == VALUES_IN_KEYS:
         return g.head_dim
     return g.head_dim + (g.value_dim or g.head_dim)
+
+
+def _kv4_row_bytes(head_dim: int) -> int:
+    """Bytes of a token's key (or value) of one head in 4 bits: half a byte a value of whole 64s, and 2 bytes a group of 32."""
+    return -(-head_dim // 64) * 36
 
 
 def _elem_size(dtype) -> int:

@@ -82,6 +82,7 @@ def run_generate(argv) -> int:
     ap.add_argument("--max-tokens", type=int, default=256)
     ap.add_argument("--kv-mem", default="4G")
     ap.add_argument("--page-size", type=int, default=16)
+    ap.add_argument("--kv-bits", type=int, default=0, help="4: keys and values in 4 bits; 0: in the compute type")
     ap.add_argument("--max-seqs", type=int, default=64)
     ap.add_argument("--max-tokens-per-step", type=int, default=512)
     ap.add_argument("--policy", default="srpt-aging")
@@ -104,7 +105,7 @@ def run_generate(argv) -> int:
     t0 = time.perf_counter()
     engine = load_engine(o.model, dtype=o.dtype, kv_mem=parse_size(o.kv_mem), page_size=o.page_size,
                          serving=ServingConfig(o.max_tokens_per_step, o.max_seqs, run_ahead=not o.no_run_ahead), policy=o.policy, aging=o.aging,
-                         stop_tokens=parse_ids(o.stop_ids), random_weights=o.random_weights, seed=o.seed)
+                         stop_tokens=parse_ids(o.stop_ids), random_weights=o.random_weights, seed=o.seed, kv_bits=o.kv_bits)
     load_s = time.perf_counter() - t0
     if o.prompt is not None:
         prompt = parse_ids(o.prompt)

@@ -28,6 +28,7 @@
 
 #include "attention_mma.cuh"
 #include "kv4.cuh"
+#include "launchers.h"
 #include "umma.cuh"
 
 namespace tie {

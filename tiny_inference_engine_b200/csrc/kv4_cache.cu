@@ -4,6 +4,7 @@
 // the other. Eight dimensions (one 32-bit word of codes, 16 bytes of bfloat16) are one thread's; four threads share a group and meet in two
 // shuffles; a token and head is one warp (half of one up to 64 dimensions), which also settles by one vote whether all its numbers are finite.
 #include "kv4.cuh"
+#include "launchers.h"
 
 namespace tie {
 

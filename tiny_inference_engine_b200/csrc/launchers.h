@@ -73,6 +73,16 @@ TIE_API int tie_attention_decode_prep(const void* qkv, long long qkv_stride, con
                                       int n_list,
                                       int split_keys, int max_splits, float* scratch, int* counters, int cluster,
                                       cudaStream_t s);
+TIE_API int tie_kv4_append(int dtype, const void* k, const void* v, long long k_stride, long long v_stride, const int* slots, void* k_codes, void* k_words,
+                           void* v_codes, void* v_words, int tokens, int kv_heads, int head_dim, int page_size, long long pages, cudaStream_t s);
+TIE_API int tie_attention_kv4(int dtype, const void* q, long long q_stride, long long tokens, const void* k_codes, const void* k_words, const void* v_codes,
+                              const void* v_words, void* out, const int* query_start, const int* context_lens, const int* block_tables, int max_blocks, int seqs,
+                              int max_queries, int q_heads, int kv_heads, int head_dim, int page_size, long long pages, int window, float scale, const int* seq_list,
+                              int n_list, int max_context, float* scratch, int* counters, cudaStream_t s);
+TIE_API int tie_attention_prompt_kv4(const void* q, long long q_stride, long long tokens, const void* k_codes, const void* k_words, const void* v_codes,
+                                     const void* v_words, void* out, const int* query_start, const int* context_lens, const int* block_tables, int max_blocks,
+                                     int n_seqs, int max_queries, int q_heads, int kv_heads, int head_dim, int page_size, long long pages, int window, float scale,
+                                     int max_keys, cudaStream_t s);
 TIE_API int tie_attention_prompt_umma(const void* q, long long q_stride, const void* k_cache, const void* v_cache, void* out,
                                       const int* query_start, const int* context_lens, const int* block_tables,
                                       int max_blocks, int n_seqs, int max_queries, int q_heads, int kv_heads, int head_dim,

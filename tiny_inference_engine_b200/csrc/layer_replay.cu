@@ -64,6 +64,7 @@ const Launcher kLaunchers[] = {
     TIE_LAUNCHER(tie_attention_rows),       TIE_LAUNCHER(tie_attention_split),      TIE_LAUNCHER(tie_attention_merge),
     TIE_LAUNCHER(tie_attention_prompt_tc),  TIE_LAUNCHER(tie_attention_decode_tc),  TIE_LAUNCHER(tie_attention_prompt_tma),
     TIE_LAUNCHER(tie_attention_decode_tma), TIE_LAUNCHER(tie_attention_prompt_umma), TIE_LAUNCHER(tie_attention_decode_prep),
+    TIE_LAUNCHER(tie_kv4_append),           TIE_LAUNCHER(tie_attention_kv4),        TIE_LAUNCHER(tie_attention_prompt_kv4),
 };
 constexpr int kNumLaunchers = static_cast<int>(sizeof(kLaunchers) / sizeof(kLaunchers[0]));
 constexpr int kMaxArgs = 40;

@@ -1957,5 +1957,5 @@ def attention_decode_kept(q, k_cache, v_cache, out, query_start, context_lens, b
 
 
 from .kv4 import (Kv4Cache, Kv4Workspace, StepArrays, TABLES_BAD_REQUEST, TABLES_NO_PAGES, TABLES_ROWS, TABLES_SHORT,  # noqa: E402, F401
-                  attention_kv4_decode, attention_kv4_prompt, kv4_append, kv4_cache, kv4_read, kv4_workspace, release_tables, step_arrays,
+                  attention_kv4_decode, attention_kv4_prompt, kv4_append, kv4_cache, kv4_read, kv4_workspace, kv4_workspace_sizes, release_tables, step_arrays,
                   step_tables)

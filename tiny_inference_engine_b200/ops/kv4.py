@@ -160,11 +160,18 @@ def kv4_read(cache: Kv4Cache, slots: torch.Tensor, k: torch.Tensor, v: torch.Ten
     call("tie_kv4_read", dtype, *planes, slots.data_ptr(), k.data_ptr(), v.data_ptr(), k_stride, v_stride, T, *sizes, stream)
 
 
+def kv4_workspace_sizes(head_dim: int) -> tuple[int, int]:
+    """(float32 numbers, int32 zeros) of a workspace for heads of this size: for callers that keep buffers of their own (both contiguous,
+    16-byte aligned)."""
+    ctas = _workspace_ctas()
+    return ctas * 16 * (-(-head_dim // 64) * 64 + 2), ctas
+
+
 def kv4_workspace(q_heads: int, kv_heads: int, head_dim: int, device="cuda") -> Kv4Workspace:
     """The workspace of `attention_kv4_decode` and `attention_kv4_prompt` for heads of these sizes, whatever the batch."""
     _need(q_heads > 0 and kv_heads > 0 and q_heads % kv_heads == 0 and 0 < head_dim <= 256, "kv4_workspace: bad sizes")
-    ctas = library().tie_attention_kv4_ctas()
-    return Kv4Workspace(torch.empty(ctas * 16 * (-(-head_dim // 64) * 64 + 2), dtype=torch.float32, device=device), torch.zeros(ctas, dtype=torch.int32, device=device))
+    floats, counters = kv4_workspace_sizes(head_dim)
+    return Kv4Workspace(torch.empty(floats, dtype=torch.float32, device=device), torch.zeros(counters, dtype=torch.int32, device=device))
 
 
 def _workspace_ctas() -> int:

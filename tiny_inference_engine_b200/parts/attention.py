@@ -2,7 +2,7 @@
 
     q, k, v = h Wq^T, h Wk^T, h Wv^T          one product with the three weights stacked
     q, k    = norm over each head (optional), then the position encoding
-    k, v    -> cache pages at this step's slots
+    k, v    -> cache pages at this step's slots (in 4 bits where the cache keeps them so: ops/kv4.py)
     out     = softmax(scale q k^T, causal, optional window) v, then Wo
 
 Formulas: src/model/qwen3.cpp:218-230 and src/backend/cpu/cpu_backend.cpp:261-319. Every
@@ -30,6 +30,7 @@ TMA_DECODE_TABLE_ENTRIES = 512     # tie_attention_decode_limit(0) (csrc/attenti
 
 class GQAttention(Mixer):
     launches_only = True
+    takes_kv4 = True
 
     def __init__(self, spec, dtype, prefix: str = ""):
         p = spec.params
@@ -106,7 +107,18 @@ class GQAttention(Mixer):
             if self._capacity is None:
                 self._capacity = (ops.partial_capacity(ctx.ws.max_rows, self.gemm_qkv.N, self.gemm_qkv.K, split_many=False),
                                   ops.partial_capacity(ctx.ws.max_rows, self.gemm_o.N, self.gemm_o.K))
-            got = (self.gemm_qkv if cache.writes else self.gemm_q)(
+            product = self.gemm_qkv if cache.writes else self.gemm_q
+            if cache.kv4 is not None:
+                product(h, qkv)
+                q, k = qkv[:, :self.q_dim], qkv[:, self.q_dim:self.q_dim + self.kv_dim]
+                ops.qk_norm_rope_append(q, qw, None, q_eps, 0.0, table, ctx.positions, None, None, None, Hq, Hkv, Dh, write_kv=False)
+                if cache.writes:
+                    ops.qk_norm_rope_append(k, kw, None, k_eps, 0.0, table, ctx.positions, None, None, None, Hkv, Hkv, Dh, write_kv=False)
+                    ops.kv4_append(k, qkv[:, self.q_dim + self.kv_dim:], g.slots, cache.kv4)
+                attn = ctx.ws.rows("attn.out", T, self.q_dim, self.dtype)
+                self.attend(q, attn, ctx, g, cache)
+                return self.output(attn, ctx)
+            got = product(
                 h, qkv, lambda n: ctx.ws.flat("attn.qkv.partial", n, torch.float32, self._capacity[0]))
             partial = got if isinstance(got, ops.SplitSum) else None
             if ctx.multi_rows == 0 and ops.attention_decode_prep_takes(qkv, Hq, Hkv, Dh, cache.k.shape[2], table):
@@ -134,7 +146,10 @@ class GQAttention(Mixer):
                     self.k_norm.rows(k.view(T * Hkv, Dh), k.view(T * Hkv, Dh))
                 if not self.position.is_identity:
                     self.position.apply(k, ctx.positions, Hkv, Dh)
-                ops.kv_append(k, v, g.slots, cache.k, cache.v)
+                if cache.kv4 is not None:
+                    ops.kv4_append(k, v, g.slots, cache.kv4)
+                else:
+                    ops.kv_append(k, v, g.slots, cache.k, cache.v)
         attn = ctx.ws.rows("attn.out", T, self.q_dim, self.dtype)
         self.attend(q, attn, ctx, g, cache)
         return self.output(attn, ctx)
@@ -151,6 +166,15 @@ class GQAttention(Mixer):
         sequence that brings one token (ctx.multi_rows, ctx.single_seqs). bfloat16 with a head
         size the tensor-core kernels take runs there, everything else on the CUDA cores."""
         Hq, Hkv, Dh = self.heads, self.kv_heads, self.head_dim
+        if cache.kv4 is not None:
+            floats, counters = ops.kv4_workspace_sizes(Dh)
+            work = ops.Kv4Workspace(ctx.ws.flat("attn.kv4", floats, torch.float32), ctx.ws.zeros("attn.kv4.counters", counters, torch.int32))
+            where = (ctx.query_start, ctx.context_lens, g.block_tables)
+            if ctx.multi_rows > 0:
+                ops.attention_kv4_prompt(q, cache.kv4, attn, *where, ctx.multi_seqs, ctx.multi_max_queries, Hq, self.scale, portion_keys(ctx), work, self.window)
+            if ctx.single_count > 0:
+                ops.attention_kv4_decode(q, cache.kv4, attn, *where, Hq, self.scale, ctx.single_seqs, ctx.single_count, ctx.single_max_context, work, self.window)
+            return
         tc = ops.attention_tc_takes(q, Hq, Hkv, Dh)
         if ctx.multi_rows > 0:
             n = ctx.multi_rows

@@ -103,6 +103,8 @@ class Mixer(Part):
     # decode steps of a model with such mixers are then captured as CUDA graphs like those of a model without state.
     # False (the default) keeps every step of the model out of graphs.
     graph_safe = False
+    # True for a mixer that takes a cache in 4 bits (`LayerCache.kv4`).
+    takes_kv4 = False
 
     def cache_need(self) -> CacheNeed | None:
         return None

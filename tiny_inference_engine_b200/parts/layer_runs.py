@@ -87,6 +87,14 @@ def unchanged(places: list) -> bool:
     return True
 
 
+def _planes(view) -> list[torch.Tensor]:
+    """The cache planes of a run entry's view, in slot order."""
+    if view is None:
+        return []
+    four = getattr(view, "kv4", None)
+    return [t for t in (four[:4] if four is not None else (view.k, view.v)) if t is not None]
+
+
 def _extent_bytes(t: torch.Tensor) -> int:
     if t.numel() == 0:
         return 0
@@ -120,7 +128,7 @@ class LayerRuns:
         self._held = []     # weak references to the layers' own tensors: one that is gone means the table is stale
         for i in range(len(order)):
             ok, scalars, tensors, view = self._entry(model, cache, i)
-            planes = sum(1 for t in ((view.k, view.v) if view is not None else ()) if t is not None)
+            planes = len(_planes(view))
             self._held += [weakref.ref(t) for t in tensors[:len(tensors) - planes]]
             if states is not None and states.tensor(i) is not None:
                 ok = False      # state of its own: one tensor per entry that is not on the layer
@@ -161,7 +169,7 @@ class LayerRuns:
         tensors, scalars = [], []
         ok = walk_part(model.layers[model.spec.run_order[i].layer], tensors, scalars, set(), places)
         view = LayerRuns._view(model, cache, i)
-        tensors += [t for t in ((view.k, view.v) if view is not None else ()) if t is not None]
+        tensors += _planes(view)
         return ok, scalars, tensors, view
 
     def spans(self, i: int, start: int):
@@ -173,14 +181,14 @@ class LayerRuns:
         known = self._looks.get((i, start))
         if known is not None and unchanged(known[0]):
             view = self._view(model, cache, i)
-            tensors = [r() for r in known[1]] + [t for t in ((view.k, view.v) if view is not None else ()) if t is not None]
+            tensors = [r() for r in known[1]] + _planes(view)
             if all(t is not None for t in tensors) and [(t.data_ptr(), t.shape, t.stride()) for t in tensors] == known[2]:
                 return known[3]
         places: list = []
         _, _, tensors, view = self._entry(model, cache, i, places)
         if len(tensors) != len(row) or any(t.data_ptr() != int(p) for t, p in zip(tensors, row)):
             return None
-        planes = sum(1 for t in ((view.k, view.v) if view is not None else ()) if t is not None)
+        planes = len(_planes(view))
         spans = [(t.data_ptr(), _extent_bytes(t)) for t in tensors]
         self._looks[i, start] = (places, [weakref.ref(t) for t in tensors[:len(tensors) - planes]],
                                  [(t.data_ptr(), t.shape, t.stride()) for t in tensors], spans)

@@ -17,11 +17,13 @@ from .layer_runs import LayerRuns, same_handoff
 
 @dataclass
 class LayerCache:
-    """What a run entry sees of the cache: its planes, its group, and whether it writes them."""
+    """What a run entry sees of the cache: its planes, its group, and whether it writes them. A cache in 4 bits has `kv4`
+    (ops.Kv4Cache) in place of `k` and `v`."""
     k: torch.Tensor | None
     v: torch.Tensor | None
     group: int
     writes: bool
+    kv4: object = None
 
 
 def _build_block(layer_spec, dtype):
