@@ -1,26 +1,30 @@
 // Attention over a cache in 4 bits (the format: kv4.cuh) for few rows at a time: sequences that bring one token, short portions, the 32-bit
-// path, and every head size up to 256. Long bfloat16 portions of heads up to 128 run in attention_prompt_kv4.cu.
+// path, and every head size up to 256. Long bfloat16 portions of heads up to 128 run in attention_prompt_umma.cu.
 //
 // What it computes, for row (query j of sequence s, head h): pos = context - queries + j, keys lo..pos (lo > 0 only with a window),
 //     out = sum_k softmax_k(scale q . K_k) V_k,   K_k, V_k the bfloat16 values that the codes stand for;  no key: zeros.
 //
 // The cache has to be read once: 9/8 head_dim bytes a token and kv head, a quarter of a bfloat16 cache's, so at the same memory rate a value has a
-// quarter of the time. What an SM can spend on one is then about two instructions of a warp for 32 values, and the kernel is laid out around
+// quarter of the time. What bounds the kernel is therefore not the memory but how many instructions a value takes, and the layout follows from
 // that:
 //   - The products run transposed, S^T = K Q^T and O^T = V^T P^T on mma.sync m16n8k16: keys (then dimensions) are the 16 rows and the
 //     query heads of a kv head the 8 columns, so eight heads fill a tile that would be half empty the other way round, and what is taken
 //     apart is the A operand, whose registers a thread makes itself out of words it loads as they lie in memory. A sum does not care about
 //     the order of its terms, so which dimension (or key) stands at which place of a tile is chosen such that every thread reads whole
 //     words: a thread of a quad a quarter of a key's row, a thread of eight an eighth of a value's.
-//   - Two codes become two bfloat16 values in three instructions: shift, (and | or) that puts the codes into the mantissa of 16, one
-//     fma with the group's s and -(16 + z) s. Every one of them is exact.
+//   - Two codes become two bfloat16 values by a mask and an fma (kv4.cuh); a shift for every other pair, or, where two keys' words are put side by
+//     side anyway, none.
 //   - The scores' accumulators have keys as rows; movmatrix turns the weights into the B operand of the second product.
+//   - Up to four rows stand in the eight columns twice, and the weights' second terms take the columns that would be empty.
 //   - The maximum moves only when a score exceeds it by 2^8 (any reference gives the same quotient), which costs one vote a tile.
-// A CTA is four warps that share (sequence, kv head, 8 or 16 rows, a split of the keys); each warp has its own 32-key tiles (every fourth of the
+// A CTA is four warps that share (sequence, kv head, 4, 8 or 16 rows, a split of the keys); each warp has its own 32-key tiles (every fourth of the
 // split) and its own ring of stages, filled by cp.async, so that warps wait for memory only, never for one another. (Bulk copies
 // of pages, one an instruction, come out slower: a warp issues them one after the other, and with pages of 16 tokens eight a tile cost more
-// instructions than the 36 of a tile's cp.asyncs and their addresses.) At the end the warps put their sums together in shared memory, and the
+// instructions than a tile's cp.asyncs and their addresses.) At the end the warps put their sums together in shared memory, and the
 // splits theirs in the workspace: the last CTA to arrive adds them in split order, so the result does not depend on who came last.
+// Measured (one B200, in a graph): 32 heads over 8 of 128, eight contexts of 32,768 keys 74 us: 302 MB at 4.1 TB/s, 0.63 of the copy rate; 64 contexts of 512
+// to 4,096 keys 52 us; one of 4,096 keys 9.7 us. Counters of the first: 175 instructions a warp for 8 keys, 2.3 instructions a cycle and
+// SM, logical pipe 50 %, fma pipe 34 %, tensor pipe 21 %: what remains is two-cycle operations that get in one another's way.
 //
 // The weights enter the second product as two bfloat16 terms (16 bits), the queries of float rows and their weights as three (24 bits):
 // the operands then have the bits that the result's type can show.
@@ -35,7 +39,7 @@ namespace tie {
 
 constexpr int kKv4Threads = 128;
 constexpr int kKv4Tile = 32;              // keys of a warp's tile
-constexpr int kKv4Stages = 3;
+constexpr int kKv4Stages = 2;
 constexpr int kKv4MaxCtas = 2368;         // CTAs that leave partial sums (the workspace's size): 16 an SM
 
 struct Kv4Args {
@@ -126,7 +130,7 @@ __global__ void __launch_bounds__(kKv4Threads, NG <= 2 && ROWS <= 8 && !F32 ? 4 
   const int G = a.q_heads / a.kv_heads;
   const int t0 = a.query_start[seq], nq = a.query_start[seq + 1] - t0, context = a.context_lens[seq];
   const int rows = min(nq * G - rb * ROWS, ROWS);
-  if (rows <= 0) return;
+  if (rows <= 0 || t0 < 0) return;
   const int pos0 = context - nq;                                           // position of the sequence's first row
   const int q_first = rb * ROWS / G, q_last = (rb * ROWS + rows - 1) / G;
   int hi = pos0 + q_last;
@@ -563,7 +567,7 @@ static int launch_attn_kv4(const Kv4Args& a, int n_list, cudaStream_t s) {
   constexpr int STAGE = 2 * kKv4Tile * 36 * NG;
   constexpr size_t smem = 4 * kKv4Stages * STAGE + (F32 ? 3 * 4 * NG * 32 * 8 : 0) + 16;
   static_assert(smem <= 227 * 1024 && !(F32 && ROWS != 8), "shared memory of one CTA");
-  if (cudaFuncSetAttribute(attn_kv4_kernel<NG, ROWS, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess) {
+  if (smem > 48 * 1024 && cudaFuncSetAttribute(attn_kv4_kernel<NG, ROWS, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess) {
     set_error("attention_kv4: cannot reserve %zu bytes of shared memory", smem);
     return kCudaError;
   }
@@ -608,7 +612,7 @@ TIE_API int tie_attention_kv4(int dtype, const void* q, long long q_stride, long
   // Splits. Few (sequence, kv head, row block)s: as many as fill the SMs once (what one SM holds at a time: four CTAs, two of the larger forms), of
   // 256 keys at least (one request at 4,096 keys, 8 kv heads: 17 splits 10.0 us, 9 splits 11.2, 34 10.7). Where not even four fit, contexts are
   // cut into pieces of 1,024 keys at least, enough for two rounds, so that the longest does not set the pace alone (64 contexts of 512 to
-  // 4,096 keys: three splits 52.7 us, one 69.0; pieces of 256 keys 58.0).
+  // 4,096 keys: three splits 53 us, one 69; pieces of 256 keys 58).
   const int places = 148 * (ng <= 2 && cta_rows <= 8 && !f32 ? 4 : 2);
   const long long ctas = x * n_list;
   const int keys = window > 0 ? (max_context < window + max_queries ? max_context : window + max_queries) : max_context;

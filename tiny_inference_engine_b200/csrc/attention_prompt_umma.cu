@@ -197,7 +197,7 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
   const int nq = a.query_start[seq + 1] - t0;
   const int rows = nq * G;
   const int row0 = (static_cast<int>(gridDim.y) - 1 - static_cast<int>(blockIdx.y)) * a.cta_rows;   // last rows (most keys) first
-  if (row0 >= rows) return;
+  if (row0 >= rows || (KV4 && t0 < 0)) return;
   const int pos0 = a.context_lens[seq] - nq;
 
   // key tiles each row tile needs: first[q]..last[q]; the CTA walks first[0]..last[1] (or last[0])
@@ -622,7 +622,7 @@ static int launch_prompt_umma(const CUtensorMap& km, const CUtensorMap& vm, cons
   constexpr size_t smem = 4 * 128 * 128 + static_cast<size_t>(STAGES) * 2 * (DH / 64) * 64 * 128 + (KV4 ? kv4_raw_bytes<DH>() : 0) + (2 * STAGES + 12) * 8 + 16 + 1024;
   static_assert(smem <= 227 * 1024, "shared memory of one CTA");
   static bool configured = false;
-  if (!configured) {
+  if (KV4 || !configured) {      // (the attribute belongs to a device: KV4 asks for it on whichever is the current one)
     if (cudaFuncSetAttribute(attn_prompt_umma_kernel<DH, STAGES, KV4>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess) {
       set_error("attention_prompt_umma: cannot reserve %zu bytes of shared memory", smem);
       return kCudaError;

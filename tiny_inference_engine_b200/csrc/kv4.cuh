@@ -4,8 +4,8 @@
 // group with lo = min(0, least) and hi = max(0, largest):
 //     s = (hi - lo) / 15 in float, at least 2^-100, rounded up to three significant bits
 //     z = rint(-lo / s),  code = clamp(rint(x / s) + z, 0, 15),  value = s (code - z)
-// |code - z| <= 15 has four bits and s three, so every value is a bfloat16 number (seven bits), and so are s (16 + z) (eight) and every
-// step on the way: the products run on the tensor cores without another rounding. The quotients by s are correctly rounded floats; for a
+// |code - z| <= 15 has four bits and s three, so every value is a bfloat16 number (seven bits), and so is s z: the products run on the tensor
+// cores without another rounding. The quotients by s are correctly rounded floats; for a
 // divisor of three bits no quotient rounds to a tie that it is not (a quotient's distance from k + 1/2, if any, is more than half its ulp), so
 // rint() gives what exact arithmetic gives.
 // Codes: padded / 2 bytes, dimension d in byte d / 2, the even one in the low bits; eight dimensions are one 32-bit word. A group's 16-bit
@@ -39,7 +39,7 @@ __device__ __forceinline__ uint32_t bf16x2_fma(uint32_t a, uint32_t b, uint32_t 
 // subnormal numbers and the first normal ones lie on one line. So a code in bits 0..3 or 4..7 of a half word is a number as it stands, once
 // the other bits are masked away, code 2^-133 or code 2^-129, and one fma with s 2^69 or s 2^65 and -z s 2^-64 makes the value times 2^-64
 // of it, exactly (the products take 2^64 back in float). Against the code put into the mantissa of 16, which takes a shift and two
-// constants: a decode step over 8 x 32,768 keys KV4_US us against 94; logical operations and shifts share the pipe that bounds these kernels.
+// constants: eight contexts of 32,768 keys 81 us against 94 (then); logical operations and shifts share the pipe that bounds these kernels.
 // Scales from 2^57 up count as 2^57, so that s 2^69 stays finite (and NaN stays NaN); values below 2^-62 lose bits.
 constexpr float kKv4Unscale = 18446744073709551616.0f;     // 2^64
 // `words`: two groups' words, one in each half (the same one twice where both numbers of a pair belong to one group).

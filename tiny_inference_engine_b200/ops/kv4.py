@@ -1,5 +1,5 @@
 """A key/value cache in 4 bits whose step tables are built on the GPU: Python faces of csrc/kv4_cache.cu, csrc/attention_kv4.cu,
-csrc/attention_prompt_kv4.cu and csrc/step_tables.cu (checks of the arguments, then one or two launches on the current stream).
+csrc/attention_prompt_umma.cu and csrc/step_tables.cu (checks of the arguments, then one or two launches on the current stream).
 
 A token's key (and value) of one kv head is `head_dim` numbers, padded with zeros to whole 64s, in groups of 32. Of a group, with
 lo = min(0, its least) and hi = max(0, its largest):
@@ -10,7 +10,8 @@ lo = min(0, its least) and hi = max(0, its largest):
 so that every value is a bfloat16 number within s of what was appended, and costs 4.5 bits. Codes lie in padded / 2 bytes, dimension d in
 byte d // 2, the even one in the low bits; a group's 16-bit word holds s as bfloat16 (its low five bits are zero) and z in its low four. A token
 and head whose key or value holds a number that is not finite, or one of magnitude 2^120 or more, gets the key words 0x7fc0, zero
-value words and zero codes: rows that see that key are NaN, no other is.
+value words and zero codes: rows that see that key are NaN, no other is. Attention reads steps s from 2^57 up as 2^57, so keys and values are
+to stay below 2^57 in magnitude; what they hold below 2^-62 it may lose.
 """
 from __future__ import annotations
 
@@ -249,7 +250,9 @@ def attention_kv4_prompt(q, cache: Kv4Cache, out, query_start, context_lens, blo
                          max_context: int, workspace: Kv4Workspace, window: int = 0) -> None:
     """Causal attention of the first n_seqs sequences of the step, each bringing up to max_queries tokens that are in the cache already: row t of
     sequence s sits at pos = context_lens[s] - (its queries) + (t - query_start[s]) and sees keys 0..pos (with a window: the last `window` of
-    them). Types, layouts and `max_context` as in `attention_kv4_decode`."""
+    them). A sequence that brings more than max_queries tokens has its first ones only, the other rows are left as they are. Types, layouts and
+    `max_context` as in `attention_kv4_decode`; bfloat16 rows of long portions (UMMA_MIN_ROWS, heads of up to 128, a multiple of 8) run on
+    tcgen05, where weights enter the value product as one bfloat16 number."""
     checked = _check_attention("attention_kv4_prompt", q, cache, out, query_start, context_lens, block_tables, q_heads, workspace, window, n_seqs, scale,
                                max_context, max_queries)
     max_queries = min(max_queries, checked[3])
