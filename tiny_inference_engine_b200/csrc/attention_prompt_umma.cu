@@ -20,7 +20,7 @@
 //             grown by more than 2^8 since the value it was last scaled for (any reference point gives
 //             the same O / sum, as long as nothing overflows).
 //   8         TMA producer: lane b fetches box b (a page, or 64 keys of a larger page) of every tile.
-//   9         one thread issues the MMAs: Q K^T of tile i + 1 ahead of P V of tile i.
+//   9         one thread issues the MMAs: for one row tile and then the other, P V of a key tile and Q K^T of the one after the next.
 // Barriers: kv_full/kv_empty per stage, and for each row tile s_full (scores written), s_empty
 // (scores read), p_full[2] (P written, O rescaled), p_empty[2] (P V retired). Every wait on an mbarrier is bounded.
 // Where the rows are few and the keys many, 2 or 4 CTAs of a thread-block cluster share out the keys of 256 rows and put their sums
@@ -177,7 +177,7 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
   constexpr float kRescaleStep = 8.0f;
 
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);      // (an offset, so that the compiler still sees shared memory)
   uint8_t* p_smem = smem;                 // [row tile][buffer]
   uint8_t* ring = p_smem + 4 * P_BYTES;
   uint8_t* raw = ring + STAGES * STAGE_BYTES;      // KV4: codes and words on their way
@@ -320,75 +320,73 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
       const uint32_t v_lo0 = desc_lo_sw128(smem_u32(ring + PLANE_BYTES), 64 * 128);   // blocks of 64 head-dim columns lie 64 rows apart
       const uint32_t p_lo0 = desc_lo_sw128(smem_u32(p_smem));
       int n_qk[2] = {0, 0}, n_pv[2] = {0, 0};
-      int s_qk = 0, s_pv = 0;
-      uint32_t parity_qk = 0;
       bool ok = true;
       // Step i: Q K^T of key tile i for both row tiles, then P V of key tile i - 1 for both. The scores of
       // tile i are asked for as soon as the softmax groups have taken those of tile i - 1 out of tensor memory
       // (early in their work on them), so they are there when the groups come back for them; P V of tile i - 1
       // has to wait for the groups to finish that tile anyway. What a step waits for it waits for at once: a
       // wait costs this one thread a couple of hundred cycles even when the barrier has long flipped.
-      for (int i = 0; i <= n_tiles && ok; ++i) {
-        if (i < n_tiles) {
-          const int t = kt_first + i;
-          const bool on0 = has[0] && t >= first[0] && t <= last[0], on1 = has[1] && t >= first[1] && t <= last[1];
-          const BarrierPhase w0{kv_full + s_qk, parity_qk, true};
-          const BarrierPhase w1{s_empty + 0, static_cast<uint32_t>((n_qk[0] & 1) ^ 1), on0};
-          const BarrierPhase w2{s_empty + 1, static_cast<uint32_t>((n_qk[1] & 1) ^ 1), on1};
-          if (!__all_sync(0xffffffffu, mbar_wait_all(w0, w1, w2, abort_flag, a.status, 12) ? 1 : 0)) break;
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t k_lo = k_lo0 + s_qk * (STAGE_BYTES >> 4);
-          if (elect_one()) {
+      const auto on = [&](int q, int i) { return has[q] && i >= 0 && i < n_tiles && kt_first + i >= first[q] && kt_first + i <= last[q]; };
+      const auto qk = [&](int q, int i) {
+        const uint32_t k_lo = k_lo0 + (i % STAGES) * (STAGE_BYTES >> 4);
+        if (elect_one()) {
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              if (!(q == 0 ? on0 : on1)) continue;
-#pragma unroll
-              for (int ks = 0; ks < DH / 16; ++ks) {
-                umma_bf16_a_tmem(tmem_base + q * kKeysPerTile, tmem_base + Q_COL + q * (DH / 2) + ks * 8,
-                                 desc_from_words(k_lo + (((ks >> 2) * (64 * 128) + (ks & 3) * 32) >> 4), kDescHiSw128), idesc_qk,
-                                 ks > 0 ? 1u : 0u);
-              }
-              umma_commit(s_full + q);
-            }
+          for (int ks = 0; ks < DH / 16; ++ks) {
+            umma_bf16_a_tmem(tmem_base + q * kKeysPerTile, tmem_base + Q_COL + q * (DH / 2) + ks * 8,
+                             desc_from_words(k_lo + (((ks >> 2) * (64 * 128) + (ks & 3) * 32) >> 4), kDescHiSw128), idesc_qk, ks > 0 ? 1u : 0u);
           }
-          __syncwarp();
-          n_qk[0] += on0 ? 1 : 0;
-          n_qk[1] += on1 ? 1 : 0;
-          if (++s_qk == STAGES) {
-            s_qk = 0;
-            parity_qk ^= 1;
-          }
+          umma_commit(s_full + q);
         }
-        if (i >= 1) {
-          const int t = kt_first + i - 1;
-          const bool on0 = has[0] && t >= first[0] && t <= last[0], on1 = has[1] && t >= first[1] && t <= last[1];
-          const int pb0 = n_pv[0] & 1, pb1 = 2 + (n_pv[1] & 1);          // the tiles' P buffers, each used for the (n_pv / 2)-th time
-          const BarrierPhase w0{p_full + pb0, static_cast<uint32_t>((n_pv[0] >> 1) & 1), on0};
-          const BarrierPhase w1{p_full + pb1, static_cast<uint32_t>((n_pv[1] >> 1) & 1), on1};
-          const BarrierPhase w2{nullptr, 0u, false};
-          if (!__all_sync(0xffffffffu, mbar_wait_all(w0, w1, w2, abort_flag, a.status, 14) ? 1 : 0)) break;
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t v_lo = v_lo0 + s_pv * (STAGE_BYTES >> 4);
-          if (elect_one()) {
+        __syncwarp();
+        ++n_qk[q];
+      };
+      const auto pv = [&](int q, int i) {
+        const uint32_t v_lo = v_lo0 + (i % STAGES) * (STAGE_BYTES >> 4);
+        const int pb = 2 * q + (n_pv[q] & 1);
+        const uint32_t p_lo = p_lo0 + pb * (P_BYTES >> 4);
+        const uint32_t keep = n_pv[q] > 0 ? 1u : 0u;
+        if (elect_one()) {
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              if (!(q == 0 ? on0 : on1)) continue;
-              const int pb = q == 0 ? pb0 : pb1;
-              const uint32_t p_lo = p_lo0 + pb * (P_BYTES >> 4);
-              const uint32_t keep = n_pv[q] > 0 ? 1u : 0u;
-#pragma unroll
-              for (int kk = 0; kk < kKeysPerTile / 16; ++kk) {
-                umma_bf16(tmem_base + O_COL + q * DH, desc_from_words(p_lo + ((kk * 32) >> 4), kDescHiSw128),
-                          desc_from_words(v_lo + ((kk * 16 * 128) >> 4), kDescHiSw128), idesc_pv, kk > 0 ? 1u : keep);
-              }
-              umma_commit(p_empty + pb);
-            }
-            umma_commit(kv_empty + s_pv);   // both products of key tile i - 1 have read the stage once everything issued so far retires
+          for (int kk = 0; kk < kKeysPerTile / 16; ++kk) {
+            umma_bf16(tmem_base + O_COL + q * DH, desc_from_words(p_lo + ((kk * 32) >> 4), kDescHiSw128),
+                      desc_from_words(v_lo + ((kk * 16 * 128) >> 4), kDescHiSw128), idesc_pv, kk > 0 ? 1u : keep);
           }
-          __syncwarp();
-          n_pv[0] += on0 ? 1 : 0;
-          n_pv[1] += on1 ? 1 : 0;
-          if (++s_pv == STAGES) s_pv = 0;
+          umma_commit(p_empty + pb);
+        }
+        __syncwarp();
+        ++n_pv[q];
+      };
+      // Step i, for row tile 0 and then for row tile 1: P V of key tile i - 1, once the softmax has written its weights, and Q K^T of key tile
+      // i + 1, once it has taken the scores of tile i, which happens right behind that. The row tiles have waits of their own, so one's products
+      // run while the other's softmax does: 8,192 tokens of 32 heads over 8 of 128 545 us, 649 with one wait for both row tiles' scores and one for
+      // their weights. A wait costs this one thread a couple of hundred cycles even when the barrier has long flipped, so a row tile's are
+      // one (two: 606 us); but with KV4 and heads of 128, whose stages are three and filled by warps, P V and the stage's release come first
+      // (694 us against 815).
+      constexpr bool TOGETHER = !KV4 || DH == 64;
+      const BarrierPhase none{nullptr, 0u, false};
+      const auto wait = [&](const BarrierPhase& w0, const BarrierPhase& w1, const BarrierPhase& w2) {
+        if (!w0.on && !w1.on && !w2.on) return;
+        ok = __all_sync(0xffffffffu, mbar_wait_all(w0, w1, w2, abort_flag, a.status, 12) ? 1 : 0) != 0;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      };
+      for (int i = -1; i <= n_tiles && ok; ++i) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const bool next = on(q, i + 1), last_one = on(q, i - 1);
+          const BarrierPhase keys{kv_full + (i + 1) % STAGES, static_cast<uint32_t>(((i + 1) / STAGES) & 1), q == 0 && i + 1 < n_tiles};
+          const BarrierPhase taken{s_empty + q, static_cast<uint32_t>((n_qk[q] & 1) ^ 1), next};
+          const BarrierPhase weights{p_full + 2 * q + (n_pv[q] & 1), static_cast<uint32_t>((n_pv[q] >> 1) & 1), last_one};
+          if (TOGETHER) wait(keys, taken, weights);
+          else wait(weights, none, none);
+          if (!ok) break;
+          if (last_one) pv(q, i - 1);
+          if (q == 1 && i >= 1) {        // both row tiles are done with key tile i - 1
+            if (elect_one()) umma_commit(kv_empty + (i - 1) % STAGES);
+            __syncwarp();
+          }
+          if (!TOGETHER) wait(keys, taken, none);
+          if (!ok) break;
+          if (next) qk(q, i + 1);
         }
       }
     }
