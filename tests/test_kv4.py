@@ -89,6 +89,10 @@ def test_attention_refuses():
     refused(ops.attention_kv4_prompt, **good, n_seqs=3, max_queries=1)
     refused(ops.attention_kv4_prompt, **good, n_seqs=2, max_queries=-1)
     refused(ops.kv4_workspace, 3, 2, 64, device="cpu")
+    refused(ops.Kv4Workspace, work.scratch.double(), work.counters)
+    refused(ops.Kv4Workspace, work.scratch[::2], work.counters)
+    refused(ops.Kv4Workspace, work.scratch[1:], work.counters)
+    refused(ops.Kv4Workspace, work.scratch, work.counters.long())
 
 
 def test_step_tables_refuse():

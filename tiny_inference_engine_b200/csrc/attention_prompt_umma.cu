@@ -657,7 +657,7 @@ static void cut_prompt_umma(UmmaPromptArgs& a, int max_queries, int n_seqs, int 
   int sms = 148;
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, 0);
   // ...; with many keys they share out the keys instead: what bounds either is the keys and values that L2 feeds the SMs, and tiles of
-  // 256 rows read them half as often. 128 rows a CTA against shares, us: two shares, 512 tokens of 32 heads over 8, heads of 128: 2,100
+  // 256 rows read them half as often. 128 rows a CTA against shares, us (with one wait for both row tiles, up to a tenth slower than now): two shares, 512 tokens of 32 heads over 8, heads of 128: 2,100
   // keys 45 / 43, 3,000 57 / 51, 8,192 131 / 100, 16,384 246 / 175 (at 1,024 24 / 29: the merge costs about 8 us); heads of 64 37 / 37,
   // 47 / 45, 111 / 92, 207 / 164. Four shares, 128 tokens: heads of 128 2,100 keys 43 / 37, 3,000 55 / 41, 8,192 126 / 65; 16 heads of 64 over
   // 4 35 / 31, 45 / 35, 104 / 57; 8 over 8 of 128 41 / 29, 53 / 31, 124 / 49.
@@ -672,9 +672,9 @@ static void cut_prompt_umma(UmmaPromptArgs& a, int max_queries, int n_seqs, int 
 // The same with KV4, by what the ways cost in tiles of 64 keys by 256 rows: the CTAs' rounds on the SMs times a CTA's tiles. Two shares of the
 // keys add the time of 8 tiles to a round, four 12 (and four CTAs of a cluster find room on about 132 of the SMs); CTAs of 128 rows take 0.86 of a
 // tile's time. How many CTAs have rows is estimated from all rows of the step, since portions differ. Against what was measured (us): portions
-// of 512, 342, 172 and 2 tokens of 16 heads of 64 over 4 at 8,192 keys: one share 172, two 97, four 153 (the rule: two); 512 tokens of
-// 32 heads of 128 over 8 at 8,192 keys 203, 115, 143 (two); 128 tokens at 4,096 keys 107, 67, 48 (four); 1,024 tokens at 4,096 keys 108, 121, 180
-// (one); eight portions of 300 to 2 tokens at 4,096 keys 198, 184, 242 (two); 300 tokens at 300 keys 18.5, 22, 43, 128 rows 16.3 (128 rows).
+// of 512, 342, 172 and 2 tokens of 16 heads of 64 over 4 at 8,192 keys: one share 170, two 96, four 151 (the rule: two); 512 tokens of
+// 32 heads of 128 over 8 at 8,192 keys 184, 107, 135 (two); 128 tokens at 4,096 keys 98, 63, 47 (four); 1,024 tokens at 4,096 keys 100, 115, 176
+// (one); eight portions of 300 to 2 tokens at 4,096 keys 184, 176, 235 (two); 300 tokens at 300 keys 17.7, 22, 42, 128 rows 16.1 (128 rows).
 static void cut_prompt_kv4(UmmaPromptArgs& a, int max_queries, int n_seqs, int max_keys) {
   const long long group = a.q_heads / a.kv_heads, max_rows = max_queries * group;
   const int keys = a.window > 0 && a.window + max_queries < max_keys ? a.window + max_queries : max_keys;

@@ -45,11 +45,19 @@ class Kv4Cache(NamedTuple):
         return self.k_codes.shape[2]
 
 
-class Kv4Workspace(NamedTuple):
-    """Where the splits of a row's keys leave their sums. Calls that run one after the other may share it (`counters` is zero between them);
-    calls that may run at the same time, in two streams or two captured graphs, need one each."""
-    scratch: torch.Tensor       # float32
-    counters: torch.Tensor      # int32, zeros
+class Kv4Workspace:
+    """Where the splits of a row's keys leave their sums: `scratch` float32 (contiguous, 16-byte aligned), `counters` int32 zeros
+    (`kv4_workspace_sizes`), looked over once, here. Calls that run one after the other may share a workspace (its counters are zero between
+    them); calls that may run at the same time, in two streams or two captured graphs, need one each."""
+    __slots__ = ("scratch", "counters", "floats", "ctas", "pointers", "device")
+
+    def __init__(self, scratch: torch.Tensor, counters: torch.Tensor):
+        if scratch.dtype is not torch.float32 or counters.dtype is not torch.int32 or not (scratch.is_contiguous() and counters.is_contiguous()) or \
+                scratch.data_ptr() & 15 or scratch.get_device() != counters.get_device():
+            raise InvalidArgument("Kv4Workspace: scratch must be contiguous float32, 16-byte aligned, counters contiguous int32, both on one device")
+        self.scratch, self.counters = scratch, counters
+        self.floats, self.ctas, self.device = scratch.numel(), counters.numel(), scratch.get_device()
+        self.pointers = scratch.data_ptr(), counters.data_ptr()
 
 
 class StepArrays(NamedTuple):
@@ -210,19 +218,19 @@ def _check_attention(what, q, cache, out, query_start, context_lens, block_table
         _fail(f"{what}: {n} of {S} sequences (at most 65,535 a call)")
     if not 0 <= window < 2 ** 30:
         _fail(f"{what}: bad window {window}")
-    scratch, counters = workspace
     ctas = _workspace_ctas()
-    if scratch.dtype is not torch.float32 or counters.dtype is not _I32 or scratch.numel() < ctas * 16 * ((sizes[1] + 63) // 64 * 64 + 2) or scratch.data_ptr() & 15 or counters.numel() < ctas or not (
-            scratch.is_contiguous() and counters.is_contiguous()):
+    if workspace.floats < ctas * 16 * ((sizes[1] + 63) // 64 * 64 + 2) or workspace.ctas < ctas:
         _fail(f"{what}: the workspace is too small (kv4_workspace makes one)")
     if not (scale > 0 and max_context >= 0 and 0 <= max_queries < 2 ** 30):
         _fail(f"{what}: the scale must be positive, max_context and max_queries not negative")
     if seq_list is None:
-        stream = _stream(what, q, out, query_start, context_lens, block_tables, scratch, counters, cache[0], cache[1], cache[2], cache[3])
+        stream = _stream(what, q, out, query_start, context_lens, block_tables, cache[0], cache[1], cache[2], cache[3])
     else:
         if seq_list.dtype is not _I32 or seq_list.dim() != 1 or not seq_list.is_contiguous() or seq_list.numel() < n:
             _fail(f"{what}: seq_list must be int32 [n_list]")
-        stream = _stream(what, q, out, query_start, context_lens, block_tables, scratch, counters, cache[0], cache[1], cache[2], cache[3], seq_list)
+        stream = _stream(what, q, out, query_start, context_lens, block_tables, cache[0], cache[1], cache[2], cache[3], seq_list)
+    if workspace.device != q.get_device():
+        _fail(f"{what}: the workspace must be on the current device")
     return dtype, planes, sizes, shape[0], q_stride, S, table_shape[1], stream
 
 
@@ -230,7 +238,7 @@ def _rows_kernel(checked, q, out, query_start, context_lens, block_tables, max_q
     dtype, planes, sizes, T, q_stride, S, columns, stream = checked
     call("tie_attention_kv4", dtype, q.data_ptr(), q_stride, T, *planes, out.data_ptr(), query_start.data_ptr(), context_lens.data_ptr(),
          block_tables.data_ptr(), columns, S, max_queries, q_heads, *sizes, window, scale, seq_list, n, min(max_context, 2 ** 30),
-         workspace[0].data_ptr(), workspace[1].data_ptr(), stream)
+         *workspace.pointers, stream)
 
 
 def attention_kv4_decode(q, cache: Kv4Cache, out, query_start, context_lens, block_tables, q_heads: int, scale: float, seq_list, n_list: int,

@@ -167,8 +167,11 @@ class GQAttention(Mixer):
         size the tensor-core kernels take runs there, everything else on the CUDA cores."""
         Hq, Hkv, Dh = self.heads, self.kv_heads, self.head_dim
         if cache.kv4 is not None:
-            floats, counters = ops.kv4_workspace_sizes(Dh)
-            work = ops.Kv4Workspace(ctx.ws.flat("attn.kv4", floats, torch.float32), ctx.ws.zeros("attn.kv4.counters", counters, torch.int32))
+            work = ctx.memo.get(("kv4_workspace", Dh))
+            if work is None:
+                floats, counters = ops.kv4_workspace_sizes(Dh)
+                work = ctx.memo["kv4_workspace", Dh] = ops.Kv4Workspace(ctx.ws.flat("attn.kv4", floats, torch.float32),
+                                                                        ctx.ws.zeros("attn.kv4.counters", counters, torch.int32))
             where = (ctx.query_start, ctx.context_lens, g.block_tables)
             if ctx.multi_rows > 0:
                 ops.attention_kv4_prompt(q, cache.kv4, attn, *where, ctx.multi_seqs, ctx.multi_max_queries, Hq, self.scale, portion_keys(ctx), work, self.window)
