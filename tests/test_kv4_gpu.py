@@ -17,7 +17,7 @@ import torch
 import plain_kv4 as plain
 from tiny_inference_engine_b200 import ops
 from tiny_inference_engine_b200.errors import TieError
-from tiny_inference_engine_b200.ops import gemm_select
+from tiny_inference_engine_b200.ops import gemm_select, kv4
 
 pytestmark = pytest.mark.gpu
 NP = {"float32": np.float32, "bfloat16": np.float32}
@@ -129,7 +129,7 @@ def test_slots_outside_of_the_cache_write_nothing():
 class Batch:
     """Sequences with random keys and values in a cache, their queries, and the answer in 64 bits."""
 
-    def __init__(self, seed, contexts, queries, heads, kv_heads, head_dim, page, dtype, window=0, loud=1.0, nan_at=()):
+    def __init__(self, seed, contexts, queries, heads, kv_heads, head_dim, page, dtype, window=0, loud=1.0, nan_at=(), pad=5):
         rng = np.random.default_rng(seed)
         self.heads, self.kv_heads, self.head_dim, self.window, self.dtype = heads, kv_heads, head_dim, window, dtype
         n, T = len(contexts), sum(queries)
@@ -170,7 +170,7 @@ class Batch:
         self.contexts, self.queries = contexts, queries
         self.args = (cuda(self.start), cuda(np.array(contexts, np.int32)), cuda(tables))
         self.work = ops.kv4_workspace(heads, kv_heads, head_dim)
-        wide = torch.zeros(T, heads * head_dim + 5, dtype=DT[dtype], device="cuda")
+        wide = torch.zeros(T, heads * head_dim + pad, dtype=DT[dtype], device="cuda")
         wide[:, :heads * head_dim] = cuda(self.q.reshape(T, -1), DT[dtype])
         self.qt = wide                                      # rows of a wider product's output
         self.out = torch.full((T, heads * head_dim), 9.0, dtype=DT[dtype], device="cuda")
@@ -181,9 +181,9 @@ class Batch:
                                  max(self.contexts) if max_context is None else max_context, self.work, window=self.window)
         return self.answer()
 
-    def prompt(self, n=None):
+    def prompt(self, n=None, max_queries=None):
         n = len(self.contexts) if n is None else n
-        ops.attention_kv4_prompt(self.qt, self.cache, self.out, *self.args, n, max(self.queries), self.heads, self.scale, max(self.contexts), self.work,
+        ops.attention_kv4_prompt(self.qt, self.cache, self.out, *self.args, n, max_queries or max(self.queries), self.heads, self.scale, max(self.contexts), self.work,
                                  window=self.window)
         return self.answer()
 
@@ -193,10 +193,13 @@ class Batch:
         assert int(self.work.counters.abs().sum()) == 0
         return self.out.float().cpu().numpy().astype(np.float64).reshape(self.want.shape)
 
-    def check(self, got, rows=slice(None), one_term=False):
+    def check(self, got, rows=slice(None), one_term=False, truncated=False):
+        """`truncated`: sums on tcgen05, whose every step may cut a unit of the running sum's last place instead of half a one. Of the scores (three
+        terms, head_dim / 16 steps each, 24 for 128) by |q| |k| scale, here below 19, times 2^-23 each: the weights are off by 2^-13 with their sum.
+        Of the values 3 keys / 16 steps, 206 for 1,100 keys: 2^-15. Together below M 2^-12."""
         want, most = self.want[rows], self.most[rows]
         if self.dtype == "float32":
-            limit = most * 2.0 ** -15 + np.abs(want) * 2.0 ** -23
+            limit = most * 2.0 ** (-12 if truncated else -15) + np.abs(want) * 2.0 ** -23
         else:
             limit = np.abs(want) * 2.0 ** -8 + most * (2.0 ** -14 + (2.0 ** -8 if one_term else 0.0))
         assert np.array_equal(np.isnan(got[rows]), np.isnan(want))
@@ -246,6 +249,44 @@ PROMPT = [([5, 2], [5, 2], 8, 2, 64, 16), ([40, 300, 7], [9, 33, 2], 8, 2, 128, 
 def test_prompt(dtype, window, contexts, queries, heads, kv_heads, head_dim, page):
     b = Batch(len(contexts) * 13 + head_dim, contexts, queries, heads, kv_heads, head_dim, page, dtype, window)
     b.check(b.prompt(), one_term=True)
+
+
+# 16-byte aligned rows, run on tcgen05 too: one CTA's row tiles full and not, keys in one, two and four shares, every width of head
+LONG = [([130], [130], 4, 4, 128, 16), ([1100, 130], [128, 130], 32, 8, 128, 32), ([700, 64, 3], [40, 64, 3], 8, 1, 64, 12), ([300], [300], 4, 2, 64, 8),
+        ([900, 40], [65, 40], 16, 2, 80, 16), ([500, 129], [200, 129], 4, 2, 192, 3), ([400, 2], [129, 2], 6, 3, 136, 64), ([333, 200, 7], [64, 200, 7], 8, 2, 256, 16),
+        ([1000], [33], 8, 2, 248, 5), ([260, 257], [256, 257], 3, 3, 40, 16), ([640], [512], 8, 4, 96, 128), ([2100], [130], 12, 4, 64, 16), ([50, 9, 0], [1, 3, 0], 8, 2, 128, 16)]
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("window", [0, 29, 300])
+@pytest.mark.parametrize("contexts,queries,heads,kv_heads,head_dim,page", LONG)
+@pytest.mark.parametrize("forced", [True, False])
+def test_long_portions(monkeypatch, forced, dtype, window, contexts, queries, heads, kv_heads, head_dim, page):
+    if forced:          # whatever the number of rows
+        monkeypatch.setattr(kv4, "UMMA_MIN_ROWS", 1)
+        monkeypatch.setattr(kv4, "UMMA_GROUPS", 0)
+    b = Batch(len(contexts) * 17 + head_dim, contexts, queries, heads, kv_heads, head_dim, page, dtype, window, pad=8)
+    b.check(b.prompt(), one_term=True, truncated=True)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+def test_long_portions_leave_the_rows_that_are_not_theirs(monkeypatch, dtype, head_dim):
+    monkeypatch.setattr(kv4, "UMMA_GROUPS", 0)
+    b = Batch(head_dim, [30, 300, 50], [30, 290, 50], 8, 2, head_dim, 16, dtype, pad=8)
+    got = b.prompt(n=2, max_queries=140)
+    b.check(got, slice(0, 170), one_term=True, truncated=True)
+    assert (got[170:] == 9.0).all()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("head_dim", [64, 128, 192])
+def test_a_key_that_is_not_finite_in_a_long_portion(monkeypatch, dtype, head_dim):
+    monkeypatch.setattr(kv4, "UMMA_GROUPS", 0)
+    b = Batch(head_dim + 1, [500, 160], [200, 160], 8, 2, head_dim, 16, dtype, nan_at=((0, 310),), pad=8)
+    got = b.prompt()
+    assert np.isnan(got[10:200, :4]).all() and np.isfinite(got[:10]).all() and np.isfinite(got[200:]).all() and np.isfinite(got[:, 4:]).all()
+    b.check(got, one_term=True, truncated=True)
 
 
 def test_prompt_leaves_the_rows_behind_its_sequences():

@@ -70,18 +70,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
   return d;
 }
-__device__ __forceinline__ float bf16_lo(uint32_t v) { return __uint_as_float(v << 16); }
-__device__ __forceinline__ float bf16_hi(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
-
-// a and b as TERMS pairs of bfloat16 numbers whose sums they are (to 8 TERMS bits).
-template <int TERMS> __device__ __forceinline__ void split_terms(float a, float b, uint32_t (&t)[TERMS]) {
-#pragma unroll
-  for (int i = 0; i < TERMS; ++i) {
-    t[i] = pack_bf16(a, b);
-    if (i + 1 < TERMS) a -= bf16_lo(t[i]), b -= bf16_hi(t[i]);
-  }
-}
-
 template <int N> __device__ __forceinline__ void lds_words(uint32_t (&r)[N], const uint8_t* p) {
   if constexpr (N % 4 == 0) {
 #pragma unroll

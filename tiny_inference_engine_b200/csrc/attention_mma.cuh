@@ -37,6 +37,18 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+__device__ __forceinline__ float bf16_lo(uint32_t v) { return __uint_as_float(v << 16); }
+__device__ __forceinline__ float bf16_hi(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
+
+// a and b as TERMS pairs of bfloat16 numbers whose sums they are (to 8 TERMS bits).
+template <int TERMS> __device__ __forceinline__ void split_terms(float a, float b, uint32_t (&t)[TERMS]) {
+#pragma unroll
+  for (int i = 0; i < TERMS; ++i) {
+    t[i] = pack_bf16(a, b);
+    if (i + 1 < TERMS) a -= bf16_lo(t[i]), b -= bf16_hi(t[i]);
+  }
+}
+
 // Where 16-byte chunk c of row r lives in a shared-memory tile whose rows hold DH bfloat16 (DH a
 // multiple of 64). Both layouts XOR the chunk index with the row, so that the 8 rows an ldmatrix
 // reads at one chunk fall into 8 different bank groups.

@@ -29,9 +29,12 @@
 // grid = (kv heads, row tiles, sequences x splits): CTAs start in that order with the last row tiles first, so the
 // tiles with the most keys of every kv head run first.
 //
-// KV4: the same over a cache in 4 bits (kv4.cuh), heads of up to 64 or 128 (a multiple of 8; what is missing is zeros) and pages of any size.
-// Four warps take the place of the TMA producer: they read codes and words a tile ahead, take them apart and write the
-// tile as TMA would have. Eight dimensions lie in it in the order 0 4 1 5 2 6 3 7, in which a word of codes comes apart; Q is put into tensor
+// KV4: the same over a cache in 4 bits (kv4.cuh), heads of up to 256 (a multiple of 8; what is missing is zeros) and pages of any size.
+// Warps take the place of the TMA producer: they read codes and words some tiles ahead, take them apart and write the
+// tile as TMA would have. Heads above 128 leave tensor memory for one row tile a CTA; so do float queries, which
+// stand there as three bfloat16 terms (24 bits), as the weights do in shared memory. 4 portions of 512 queries at 2,048 keys, 32 heads over 8,
+// us against the kernel whose warps take 16 rows each: heads of 128 105 and 396 (float 205 and 646), of 64 92 and 267 (162 and 407), of 192
+// 203 and 589, of 256 330 and 790. Eight dimensions lie in a tile in the order 0 4 1 5 2 6 3 7, in which a word of codes comes apart; Q is put into tensor
 // memory in the same order and the outputs are taken out of it again. Keys and values are exact in bfloat16, times 2^-64 (kv4.cuh).
 #include "attention_mma.cuh"
 #include "kv4.cuh"
@@ -40,7 +43,6 @@
 
 namespace tie {
 
-constexpr int kUmmaAttnThreads = 320, kUmmaKv4Threads = 384;
 constexpr int kUmmaMaxSplits = 4;
 constexpr int kUmmaSplitKeys = 2049;
 
@@ -62,25 +64,52 @@ struct UmmaPromptArgs {
   // KV4 only
   const uint8_t *k_codes, *v_codes;
   const uint16_t *k_words, *v_words;
-  int head_dim, pages;
+  int head_dim, pages, max_queries;
   long long tokens;       // rows of q and out
 };
 
-// What the three producer warps of a CTA do (KV4; a fourth would leave the softmax's 64 scores a thread too few registers); `id` is 0..95 of
-// their threads. A thread takes 32 dimensions (16 bytes of codes, one group) of some keys and values of every tile. It copies them with cp.async into places of shared memory that are its own, kKv4Ahead tiles ahead, so
+// Eight outputs of a row from element `at` on; a row's start is 16-byte aligned.
+template <bool F32>
+__device__ __forceinline__ void store8(__nv_bfloat16* out, long long at, const float (&v)[8]) {
+  if constexpr (F32) {
+    float* dst = reinterpret_cast<float*>(out) + at;
+    *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4*>(dst + 4) = make_float4(v[4], v[5], v[6], v[7]);
+  } else {
+    *reinterpret_cast<uint4*>(out + at) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+  }
+}
+
+// The form of a kernel: heads of up to DH; RT row tiles of 128 a CTA; F32: float queries and outputs, in three bfloat16 terms.
+template <int DH_, bool KV4_, int RT_, bool F32_>
+struct UmmaForm {
+  static constexpr int DH = DH_, RT = RT_, TERMS = F32_ ? 3 : 1;
+  static constexpr bool KV4 = KV4_, F32 = F32_;
+  // (KV4: with one warp more the softmax's 64 scores a thread would have too few registers)
+  static constexpr int THREADS = !KV4 ? 320 : RT == 2 ? 384 : 352;
+  static constexpr int PRODUCERS = RT == 2 ? 96 : 192;            // threads that take a KV4 tile apart
+  static constexpr int STAGES = DH <= 64 ? (F32 ? 4 : 6) : DH == 128 ? (KV4 ? 3 : 4) : DH == 192 ? 3 : 2;
+  static constexpr int AHEAD = RT == 2 ? 3 : 2;                   // tiles that a producer copies ahead
+  static constexpr int ROUNDS = (kKeysPerTile * DH / 32 + PRODUCERS - 1) / PRODUCERS;     // keys (and values) of a producer thread in a tile
+  static constexpr int RAW = ROUNDS * PRODUCERS * 40;             // bytes of a tile on its way: a thread's two times 16 bytes of codes and two words
+  static constexpr int P_BYTES = 128 * 128;                       // 128 rows x 64 keys
+  static constexpr int STAGE_BYTES = 2 * (DH / 64) * 64 * 128;    // keys and values of a tile
+  static constexpr int P_ALL = RT * 2 * TERMS * P_BYTES;          // [row tile][buffer][term]
+  static constexpr int SMEM = P_ALL + STAGES * STAGE_BYTES + (KV4 ? AHEAD * RAW : 0) + (2 * STAGES + 12) * 8 + 16 + 1024;
+  static_assert(SMEM <= 227 * 1024, "shared memory of one CTA");
+  static_assert(SMEM >= RT * 128 * (DH + 4) * 4 + (2 * STAGES + 12) * 8 + 16 + 1024, "the sums of a CTA's rows");
+};
+
+// What the producer warps of a CTA do (KV4); `id` numbers their threads. A thread takes 32 dimensions (16 bytes of codes, one group) of
+// some keys and values of every tile. It copies them with cp.async into places of shared memory that are its own, AHEAD tiles ahead, so
 // nobody has to be told when they have landed; their pages it looks up another tile ahead.
-constexpr int kKv4Producers = 96, kKv4Ahead = 3;
-constexpr int kKv4RawBytes = 40;                                  // of a thread's key and value: two times 16 bytes of codes and two words
-template <int DH> constexpr int kv4_rounds() { return (kKeysPerTile * DH / 32 + kKv4Producers - 1) / kKv4Producers; }
-template <int DH> constexpr int kv4_raw_bytes() { return kKv4Ahead * kv4_rounds<DH>() * kKv4Producers * kKv4RawBytes; }
-template <int DH, int STAGES>
+template <typename Form>
 __device__ __forceinline__ void kv4_produce(const UmmaPromptArgs& a, uint8_t* ring, uint8_t* raw, uint64_t* kv_full, uint64_t* kv_empty, volatile int* abort_flag,
                                             int id, int seq, int kvh, int kt_first, int n_tiles, int lo, int hi) {
-  constexpr int GROUPS = DH / 32, PER = kv4_rounds<DH>();         // groups of a key; keys (and values) of a thread
-  constexpr int PLANE_BYTES = DH / 64 * 64 * 128, RAW = PER * kKv4Producers * kKv4RawBytes;
-  static_assert(kKv4Producers % GROUPS == 0, "a thread's keys have one group");
+  constexpr int GROUPS = Form::DH / 32, PER = Form::ROUNDS, RAW = Form::RAW, STAGES = Form::STAGES, PLANE_BYTES = Form::STAGE_BYTES / 2;
+  static_assert(Form::PRODUCERS % GROUPS == 0, "a thread's keys have one group");
   const int group = id % GROUPS, first = id / GROUPS;            // keys first + j * STEP of a tile, below its 64
-  constexpr int STEP = kKv4Producers / GROUPS;
+  constexpr int STEP = Form::PRODUCERS / GROUPS;
   const int* table = a.block_tables + static_cast<long long>(seq) * a.max_blocks;
   const uint32_t signs = kv4_signs();
   int rows[PER];                  // of the tile that is copied next; what no row sees is row 0, and masked below
@@ -98,12 +127,12 @@ __device__ __forceinline__ void kv4_produce(const UmmaPromptArgs& a, uint8_t* ri
   };
   const auto copy = [&](int i) {
     if (i < n_tiles) {
-      const uint32_t dst = smem_u32(raw + (i % kKv4Ahead) * RAW);
+      const uint32_t dst = smem_u32(raw + (i % Form::AHEAD) * RAW);
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
         if (first + j * STEP >= kKeysPerTile) break;
         const long long at = static_cast<long long>(rows[j]) * GROUPS + group;
-        const uint32_t codes = dst + (j * kKv4Producers + id) * 32, words = dst + PER * kKv4Producers * 32 + (j * kKv4Producers + id) * 8;
+        const uint32_t codes = dst + (j * Form::PRODUCERS + id) * 32, words = dst + PER * Form::PRODUCERS * 32 + (j * Form::PRODUCERS + id) * 8;
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(codes), "l"(a.k_codes + at * 16) : "memory");
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(codes + 16), "l"(a.v_codes + at * 16) : "memory");
         asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(words), "l"(a.k_words + (at & ~1LL)) : "memory");          // two groups' words
@@ -125,28 +154,28 @@ __device__ __forceinline__ void kv4_produce(const UmmaPromptArgs& a, uint8_t* ri
   };
   find(0);
 #pragma unroll 1
-  for (int i = 0; i < kKv4Ahead; ++i) {
+  for (int i = 0; i < Form::AHEAD; ++i) {
     copy(i);
     find(i + 1);
   }
 #pragma unroll 1
   for (int i = 0; i < n_tiles; ++i) {
     const int st = i % STAGES;
-    asm volatile("cp.async.wait_group %0;" ::"n"(kKv4Ahead - 1) : "memory");
-    const uint8_t* src = raw + (i % kKv4Ahead) * RAW;
+    asm volatile("cp.async.wait_group %0;" ::"n"(Form::AHEAD - 1) : "memory");
+    const uint8_t* src = raw + (i % Form::AHEAD) * RAW;
     uint4 kc[PER], vc[PER];
     uint2 words[PER];
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
       const int key = (kt_first + i) * kKeysPerTile + first + j * STEP;
       if (first + j * STEP >= kKeysPerTile) break;
-      kc[j] = *reinterpret_cast<const uint4*>(src + (j * kKv4Producers + id) * 32);
-      vc[j] = *reinterpret_cast<const uint4*>(src + (j * kKv4Producers + id) * 32 + 16);
-      words[j] = *reinterpret_cast<const uint2*>(src + PER * kKv4Producers * 32 + (j * kKv4Producers + id) * 8);
+      kc[j] = *reinterpret_cast<const uint4*>(src + (j * Form::PRODUCERS + id) * 32);
+      vc[j] = *reinterpret_cast<const uint4*>(src + (j * Form::PRODUCERS + id) * 32 + 16);
+      words[j] = *reinterpret_cast<const uint2*>(src + PER * Form::PRODUCERS * 32 + (j * Form::PRODUCERS + id) * 8);
       if (key < lo || key > hi) words[j] = make_uint2(0u, 0u);       // what no row sees: zeros
     }
-    copy(i + kKv4Ahead);          // (this thread's own place, whose words it holds)
-    find(i + kKv4Ahead + 1);
+    copy(i + Form::AHEAD);          // (this thread's own place, whose words it holds)
+    find(i + Form::AHEAD + 1);
     if (!__all_sync(0xffffffffu, mbar_wait(kv_empty + st, ((i / STAGES) & 1) ^ 1, abort_flag, a.status, 11) ? 1 : 0)) break;
     uint8_t* k_plane = ring + st * 2 * PLANE_BYTES;
 #pragma unroll
@@ -162,26 +191,27 @@ __device__ __forceinline__ void kv4_produce(const UmmaPromptArgs& a, uint8_t* ri
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-template <int DH, int STAGES, bool KV4>
-__global__ void __launch_bounds__(KV4 ? kUmmaKv4Threads : kUmmaAttnThreads, 1)
+template <typename Form>
+__global__ void __launch_bounds__(Form::THREADS, 1)
 attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, UmmaPromptArgs a) {
   pdl_sync();
-  constexpr int HALVES = DH / 64;
-  constexpr int P_BYTES = 128 * 128;              // 128 rows x 64 keys
-  constexpr int PLANE_BYTES = HALVES * 64 * 128;  // 64 keys
-  constexpr int STAGE_BYTES = 2 * PLANE_BYTES;
-  constexpr int Q_COL = 128;                      // columns 0..127: the two score tiles; then Q of both tiles (two
-  constexpr int O_COL = Q_COL + DH;               // elements a column); then the two accumulators
+  constexpr int DH = Form::DH, STAGES = Form::STAGES, RT = Form::RT, TERMS = Form::TERMS;
+  constexpr bool KV4 = Form::KV4, F32 = Form::F32;
+  constexpr int HALVES = DH / 64, P_BYTES = Form::P_BYTES, STAGE_BYTES = Form::STAGE_BYTES;
+  constexpr int PLANE_BYTES = STAGE_BYTES / 2;    // 64 keys
+  // columns: the row tiles' scores, their Q (two elements a column, a term behind the other), their accumulators; of one row tile the
+  // accumulator first
+  constexpr int S_COL = RT == 1 ? DH : 0, Q_COL = S_COL + 64 * RT, O_COL = RT == 1 ? 0 : Q_COL + RT * TERMS * DH / 2;
   constexpr uint32_t TMEM_COLS = 512;
-  static_assert(O_COL + 2 * DH <= 512, "tensor memory");
+  static_assert(64 * RT + RT * TERMS * DH / 2 + RT * DH <= 512, "tensor memory");
   constexpr float kRescaleStep = 8.0f;
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);      // (an offset, so that the compiler still sees shared memory)
-  uint8_t* p_smem = smem;                 // [row tile][buffer]
-  uint8_t* ring = p_smem + 4 * P_BYTES;
+  uint8_t* p_smem = smem;                 // [row tile][buffer][term]
+  uint8_t* ring = p_smem + Form::P_ALL;
   uint8_t* raw = ring + STAGES * STAGE_BYTES;      // KV4: codes and words on their way
-  uint64_t* kv_full = reinterpret_cast<uint64_t*>(raw + (KV4 ? kv4_raw_bytes<DH>() : 0));
+  uint64_t* kv_full = reinterpret_cast<uint64_t*>(raw + (KV4 ? Form::AHEAD * Form::RAW : 0));
   uint64_t* kv_empty = kv_full + STAGES;
   uint64_t* s_full = kv_empty + STAGES;   // [2]
   uint64_t* s_empty = s_full + 2;
@@ -195,7 +225,7 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
   const int G = a.q_heads / a.kv_heads;
   const int t0 = a.query_start[seq];
   const int nq = a.query_start[seq + 1] - t0;
-  const int rows = nq * G;
+  const int rows = (KV4 ? min(nq, a.max_queries) : nq) * G;
   const int row0 = (static_cast<int>(gridDim.y) - 1 - static_cast<int>(blockIdx.y)) * a.cta_rows;   // last rows (most keys) first
   if (row0 >= rows || (KV4 && t0 < 0)) return;
   const int pos0 = a.context_lens[seq] - nq;
@@ -227,7 +257,7 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(kv_full + s, KV4 ? kKv4Producers / 32 : 1);
+      mbar_init(kv_full + s, KV4 ? Form::PRODUCERS / 32 : 1);
       mbar_init(kv_empty + s, 1);
     }
     for (int q = 0; q < 2; ++q) {
@@ -249,29 +279,43 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem_base = *tmem_holder;
-  if (warp < 8) {
+  if (warp < 4 * RT) {
     // Q: every softmax thread puts its own row into tensor memory (rows beyond the sequence: zeros)
     const int q = warp >> 2, rr = (warp & 3) * 32 + lane;
     const int row = row0 + 128 * q + rr;
     const int head_dim = KV4 ? a.head_dim : DH;
-    const uint4* src = row < rows && (!KV4 || t0 + row / G < a.tokens)
-                           ? reinterpret_cast<const uint4*>(a.q + static_cast<long long>(t0 + row / G) * a.q_stride + static_cast<long long>(kvh * G + row % G) * head_dim)
-                           : nullptr;
-    const uint32_t q_tmem = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16) + Q_COL + q * (DH / 2);
+    const bool there = row < rows && (!KV4 || t0 + row / G < a.tokens);
+    const long long at = there ? static_cast<long long>(t0 + row / G) * a.q_stride + static_cast<long long>(kvh * G + row % G) * head_dim : 0;
+    const uint32_t q_tmem = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16) + Q_COL + q * TERMS * (DH / 2);
 #pragma unroll
     for (int c0 = 0; c0 < DH / 2; c0 += 16) {
-      uint32_t w[16];
+      uint32_t w[TERMS][16];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const uint4 v = src && (!KV4 || 2 * c0 + 8 * e < head_dim) ? src[c0 / 4 + e] : make_uint4(0u, 0u, 0u, 0u);
-        if constexpr (KV4) {        // dimensions 0 4 1 5 2 6 3 7
-          w[4 * e] = __byte_perm(v.x, v.z, 0x5410), w[4 * e + 1] = __byte_perm(v.x, v.z, 0x7632);
-          w[4 * e + 2] = __byte_perm(v.y, v.w, 0x5410), w[4 * e + 3] = __byte_perm(v.y, v.w, 0x7632);
+        const bool some = there && (!KV4 || 2 * c0 + 8 * e < head_dim);
+        if constexpr (F32) {
+          float x[8] = {};
+          if (some) load4(reinterpret_cast<const float*>(a.q) + at + 2 * c0 + 8 * e, reinterpret_cast<float(&)[4]>(x[0])),
+                    load4(reinterpret_cast<const float*>(a.q) + at + 2 * c0 + 8 * e + 4, reinterpret_cast<float(&)[4]>(x[4]));
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {             // dimensions 0 4 1 5 2 6 3 7
+            uint32_t terms[TERMS];
+            split_terms<TERMS>(x[y], x[y + 4], terms);
+#pragma unroll
+            for (int term = 0; term < TERMS; ++term) w[term][4 * e + y] = terms[term];
+          }
         } else {
-          w[4 * e] = v.x, w[4 * e + 1] = v.y, w[4 * e + 2] = v.z, w[4 * e + 3] = v.w;
+          const uint4 v = some ? reinterpret_cast<const uint4*>(a.q + at)[c0 / 4 + e] : make_uint4(0u, 0u, 0u, 0u);
+          if constexpr (KV4) {        // dimensions 0 4 1 5 2 6 3 7
+            w[0][4 * e] = __byte_perm(v.x, v.z, 0x5410), w[0][4 * e + 1] = __byte_perm(v.x, v.z, 0x7632);
+            w[0][4 * e + 2] = __byte_perm(v.y, v.w, 0x5410), w[0][4 * e + 3] = __byte_perm(v.y, v.w, 0x7632);
+          } else {
+            w[0][4 * e] = v.x, w[0][4 * e + 1] = v.y, w[0][4 * e + 2] = v.z, w[0][4 * e + 3] = v.w;
+          }
         }
       }
-      tmem_st16(q_tmem + c0, w);
+#pragma unroll
+      for (int term = 0; term < TERMS; ++term) tmem_st16(q_tmem + term * (DH / 2) + c0, w[term]);
     }
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
   }
@@ -279,9 +323,9 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 
-  if (KV4 && warp != 9 && warp >= 8) {
+  if (KV4 && warp != 9 && warp >= 4 * RT) {
     const int hi = pos0 + min(rows - 1, row0 + a.cta_rows - 1) / G, lo = a.window > 0 ? max(0, pos0 + row0 / G - a.window + 1) : 0;
-    kv4_produce<DH, STAGES>(a, ring, raw, kv_full, kv_empty, abort_flag, (warp == 8 ? 0 : warp - 9) * 32 + lane, seq, kvh, kt_first, n_tiles, lo, hi);
+    kv4_produce<Form>(a, ring, raw, kv_full, kv_empty, abort_flag, (warp - 4 * RT - (warp > 9 ? 1 : 0)) * 32 + lane, seq, kvh, kt_first, n_tiles, lo, hi);
   } else if (!KV4 && warp == 8) {
     // ---- producer
     const int box_rows = min(a.page_size, kKeysPerTile);
@@ -321,19 +365,18 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
       const uint32_t p_lo0 = desc_lo_sw128(smem_u32(p_smem));
       int n_qk[2] = {0, 0}, n_pv[2] = {0, 0};
       bool ok = true;
-      // Step i: Q K^T of key tile i for both row tiles, then P V of key tile i - 1 for both. The scores of
-      // tile i are asked for as soon as the softmax groups have taken those of tile i - 1 out of tensor memory
-      // (early in their work on them), so they are there when the groups come back for them; P V of tile i - 1
-      // has to wait for the groups to finish that tile anyway. What a step waits for it waits for at once: a
-      // wait costs this one thread a couple of hundred cycles even when the barrier has long flipped.
       const auto on = [&](int q, int i) { return has[q] && i >= 0 && i < n_tiles && kt_first + i >= first[q] && kt_first + i <= last[q]; };
       const auto qk = [&](int q, int i) {
         const uint32_t k_lo = k_lo0 + (i % STAGES) * (STAGE_BYTES >> 4);
         if (elect_one()) {
 #pragma unroll
-          for (int ks = 0; ks < DH / 16; ++ks) {
-            umma_bf16_a_tmem(tmem_base + q * kKeysPerTile, tmem_base + Q_COL + q * (DH / 2) + ks * 8,
-                             desc_from_words(k_lo + (((ks >> 2) * (64 * 128) + (ks & 3) * 32) >> 4), kDescHiSw128), idesc_qk, ks > 0 ? 1u : 0u);
+          for (int term = TERMS - 1; term >= 0; --term) {
+#pragma unroll
+            for (int ks = 0; ks < DH / 16; ++ks) {
+              umma_bf16_a_tmem(tmem_base + S_COL + q * kKeysPerTile, tmem_base + Q_COL + (q * TERMS + term) * (DH / 2) + ks * 8,
+                               desc_from_words(k_lo + (((ks >> 2) * (64 * 128) + (ks & 3) * 32) >> 4), kDescHiSw128), idesc_qk,
+                               ks > 0 || term < TERMS - 1 ? 1u : 0u);
+            }
           }
           umma_commit(s_full + q);
         }
@@ -343,13 +386,16 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
       const auto pv = [&](int q, int i) {
         const uint32_t v_lo = v_lo0 + (i % STAGES) * (STAGE_BYTES >> 4);
         const int pb = 2 * q + (n_pv[q] & 1);
-        const uint32_t p_lo = p_lo0 + pb * (P_BYTES >> 4);
+        const uint32_t p_lo = p_lo0 + pb * (TERMS * P_BYTES >> 4);
         const uint32_t keep = n_pv[q] > 0 ? 1u : 0u;
         if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < kKeysPerTile / 16; ++kk) {
-            umma_bf16(tmem_base + O_COL + q * DH, desc_from_words(p_lo + ((kk * 32) >> 4), kDescHiSw128),
-                      desc_from_words(v_lo + ((kk * 16 * 128) >> 4), kDescHiSw128), idesc_pv, kk > 0 ? 1u : keep);
+          for (int term = TERMS - 1; term >= 0; --term) {
+#pragma unroll
+            for (int kk = 0; kk < kKeysPerTile / 16; ++kk) {
+              umma_bf16(tmem_base + O_COL + q * DH, desc_from_words(p_lo + ((term * P_BYTES + kk * 32) >> 4), kDescHiSw128),
+                        desc_from_words(v_lo + ((kk * 16 * 128) >> 4), kDescHiSw128), idesc_pv, kk > 0 || term < TERMS - 1 ? 1u : keep);
+            }
           }
           umma_commit(p_empty + pb);
         }
@@ -362,7 +408,7 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
       // their weights. A wait costs this one thread a couple of hundred cycles even when the barrier has long flipped, so a row tile's are
       // one (two: 606 us); but with KV4 and heads of 128, whose stages are three and filled by warps, P V and the stage's release come first
       // (694 us against 815).
-      constexpr bool TOGETHER = !KV4 || DH == 64;
+      constexpr bool TOGETHER = !KV4 || (DH == 64 && RT == 2);
       const BarrierPhase none{nullptr, 0u, false};
       const auto wait = [&](const BarrierPhase& w0, const BarrierPhase& w1, const BarrierPhase& w2) {
         if (!w0.on && !w1.on && !w2.on) return;
@@ -371,7 +417,7 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
       };
       for (int i = -1; i <= n_tiles && ok; ++i) {
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
+        for (int q = 0; q < RT; ++q) {
           const bool next = on(q, i + 1), last_one = on(q, i - 1);
           const BarrierPhase keys{kv_full + (i + 1) % STAGES, static_cast<uint32_t>(((i + 1) / STAGES) & 1), q == 0 && i + 1 < n_tiles};
           const BarrierPhase taken{s_empty + q, static_cast<uint32_t>((n_qk[q] & 1) ^ 1), next};
@@ -380,7 +426,7 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
           else wait(weights, none, none);
           if (!ok) break;
           if (last_one) pv(q, i - 1);
-          if (q == 1 && i >= 1) {        // both row tiles are done with key tile i - 1
+          if (q == RT - 1 && i >= 1) {        // all row tiles are done with key tile i - 1
             if (elect_one()) umma_commit(kv_empty + (i - 1) % STAGES);
             __syncwarp();
           }
@@ -399,9 +445,9 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
     // take the whole warp through the masks in every tile (portions of 512, 512, 512 and 2 tokens at 8,192 keys 344 us instead of 173).
     const int pos = pos0 + min(row, rows - 1) / G;
     const uint32_t lane_base = static_cast<uint32_t>(wq * 32) << 16;
-    const uint32_t s_tmem = tmem_base + lane_base + q * kKeysPerTile;
+    const uint32_t s_tmem = tmem_base + lane_base + S_COL + q * kKeysPerTile;
     const uint32_t o_tmem = tmem_base + lane_base + O_COL + q * DH;
-    uint8_t* p_rows = p_smem + 2 * q * P_BYTES + rr * 128;
+    uint8_t* p_rows = p_smem + 2 * q * TERMS * P_BYTES + rr * 128;
     float m_run = -INFINITY, m_used = -INFINITY, l = 0.0f;
     bool ok = has[q];
     const int my_tiles = has[q] ? last[q] - first[q] + 1 : 0;
@@ -473,25 +519,47 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
       }
       const float base = m_used == -INFINITY ? 0.0f : m_used;
       float sum4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int c = 0; c < 64; c += 8) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float p0 = ex2(fmaf(__uint_as_float(sr[c + 2 * e]), a.scale_log2, -base));
-          const float p1 = ex2(fmaf(__uint_as_float(sr[c + 2 * e + 1]), a.scale_log2, -base));
-          sum4[e] += p0 + p1;
-          sr[(c >> 1) + e] = pack_bf16(p0, p1);
-        }
-      }
-      l += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
       // this buffer held P of the tile before the last one: its P V has to have retired
       const int pb = 2 * q + (n & 1);
-      ok = __all_sync(0xffffffffu, mbar_wait(p_empty + pb, ((n >> 1) & 1) ^ 1, abort_flag, a.status, 13) ? 1 : 0) != 0;
-      if (!ok) break;
-      uint8_t* p_row = p_rows + (n & 1) * P_BYTES;
+      uint8_t* p_row = p_rows + (n & 1) * TERMS * P_BYTES;
+      if constexpr (F32) {
+        ok = __all_sync(0xffffffffu, mbar_wait(p_empty + pb, ((n >> 1) & 1) ^ 1, abort_flag, a.status, 13) ? 1 : 0) != 0;
+        if (!ok) break;
 #pragma unroll
-      for (int c = 0; c < 8; ++c)
-        *reinterpret_cast<uint4*>(p_row + ((c ^ (rr & 7)) << 4)) = make_uint4(sr[4 * c], sr[4 * c + 1], sr[4 * c + 2], sr[4 * c + 3]);
+        for (int c = 0; c < 8; ++c) {
+          uint32_t w[TERMS][4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float p0 = ex2(fmaf(__uint_as_float(sr[8 * c + 2 * e]), a.scale_log2, -base));
+            const float p1 = ex2(fmaf(__uint_as_float(sr[8 * c + 2 * e + 1]), a.scale_log2, -base));
+            sum4[e] += p0 + p1;
+            uint32_t terms[TERMS];
+            split_terms<TERMS>(p0, p1, terms);
+#pragma unroll
+            for (int term = 0; term < TERMS; ++term) w[term][e] = terms[term];
+          }
+#pragma unroll
+          for (int term = 0; term < TERMS; ++term)
+            *reinterpret_cast<uint4*>(p_row + term * P_BYTES + ((c ^ (rr & 7)) << 4)) = make_uint4(w[term][0], w[term][1], w[term][2], w[term][3]);
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < 64; c += 8) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float p0 = ex2(fmaf(__uint_as_float(sr[c + 2 * e]), a.scale_log2, -base));
+            const float p1 = ex2(fmaf(__uint_as_float(sr[c + 2 * e + 1]), a.scale_log2, -base));
+            sum4[e] += p0 + p1;
+            sr[(c >> 1) + e] = pack_bf16(p0, p1);
+          }
+        }
+        ok = __all_sync(0xffffffffu, mbar_wait(p_empty + pb, ((n >> 1) & 1) ^ 1, abort_flag, a.status, 13) ? 1 : 0) != 0;
+        if (!ok) break;
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          *reinterpret_cast<uint4*>(p_row + ((c ^ (rr & 7)) << 4)) = make_uint4(sr[4 * c], sr[4 * c + 1], sr[4 * c + 2], sr[4 * c + 3]);
+      }
+      l += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
@@ -506,7 +574,7 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
       // The CTAs of the cluster leave their sums, references and row sums in shared memory (once neither row tile's products read there any
       // more); every CTA puts together a slice of the columns of all rows.
       float* const sums = reinterpret_cast<float*>(smem) + (128 * q + rr) * (DH + 4);
-      asm volatile("bar.sync 1, 256;" ::: "memory");
+      asm volatile("bar.sync 1, %0;" ::"n"(128 * RT) : "memory");
       if (mine) {
 #pragma unroll 1
         for (int c0 = 0; c0 < DH; c0 += 16) {
@@ -522,21 +590,19 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
     } else if (mine) {
       const float inv = KV4 ? (l == 0.0f ? 0.0f : kKv4Unscale / l) : l > 0.0f ? 1.0f / l : 0.0f;
       const int head_dim = KV4 ? a.head_dim : DH;
-      __nv_bfloat16* o_row = row < rows && (!KV4 || t0 + row / G < a.tokens) ? a.out + (static_cast<long long>(t0 + row / G) * a.q_heads + kvh * G + row % G) * head_dim : nullptr;
+      const bool there = row < rows && (!KV4 || t0 + row / G < a.tokens);
+      const long long at = there ? (static_cast<long long>(t0 + row / G) * a.q_heads + kvh * G + row % G) * head_dim : 0;
 #pragma unroll 1
       for (int c0 = 0; c0 < DH; c0 += 16) {
         uint32_t o[16];
         tmem_ld16(o_tmem + c0, o);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-        if (o_row) {
-          uint32_t w[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int c = KV4 ? ordered(2 * e) : 2 * e, d = KV4 ? ordered(2 * e + 1) : 2 * e + 1;
-            w[e] = pack_bf16(__uint_as_float(o[c]) * inv, __uint_as_float(o[d]) * inv);
-          }
-          if (!KV4 || c0 < head_dim) *reinterpret_cast<uint4*>(o_row + c0) = make_uint4(w[0], w[1], w[2], w[3]);
-          if (!KV4 || c0 + 8 < head_dim) *reinterpret_cast<uint4*>(o_row + c0 + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+        for (int h = 0; h < 16; h += 8) {
+          float v[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(o[h + (KV4 ? ordered(e) : e)]) * inv;
+          if (there && (!KV4 || c0 + h < head_dim)) store8<F32>(a.out, at + c0 + h, v);
         }
       }
     }
@@ -544,7 +610,7 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
   if (a.splits > 1) {
     __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-    if (warp < 8) {
+    if (warp < 4 * RT) {
       const int row = row0 + threadIdx.x;
       const uint32_t here = smem_u32(reinterpret_cast<float*>(smem) + threadIdx.x * (DH + 4));
       auto peer = [&](int r, int column) {
@@ -576,7 +642,7 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
       const int cols = DH / a.splits;
       const int head_dim = KV4 ? a.head_dim : DH;
       if (row < rows && (!KV4 || t0 + row / G < a.tokens)) {
-        __nv_bfloat16* dst = a.out + (static_cast<long long>(t0 + row / G) * a.q_heads + kvh * G + row % G) * head_dim;
+        const long long at = (static_cast<long long>(t0 + row / G) * a.q_heads + kvh * G + row % G) * head_dim;
         for (int c = rank * cols; c < (rank + 1) * cols; c += 8) {
           float v[8] = {};
 #pragma unroll
@@ -590,10 +656,10 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
               for (int y = 0; y < 4; ++y) v[e + y] = fmaf(x[y], f[r] * inv, v[e + y]);
             }
           }
-          uint32_t w[4];
+          float o[8];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) w[e] = pack_bf16(v[KV4 ? ordered(2 * e) : 2 * e], v[KV4 ? ordered(2 * e + 1) : 2 * e + 1]);
-          if (!KV4 || c < head_dim) *reinterpret_cast<uint4*>(dst + c) = make_uint4(w[0], w[1], w[2], w[3]);
+          for (int e = 0; e < 8; ++e) o[e] = v[KV4 ? ordered(e) : e];
+          if (!KV4 || c < head_dim) store8<F32>(a.out, at + c, o);
         }
       }
     }
@@ -613,30 +679,27 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
   }
 }
 
-template <int DH, bool KV4>
+template <typename Form>
 static int launch_prompt_umma(const CUtensorMap& km, const CUtensorMap& vm, const UmmaPromptArgs& a, int n_seqs, int max_rows,
                               cudaStream_t s) {
-  constexpr int STAGES = DH == 128 ? (KV4 ? 3 : 4) : 6, THREADS = KV4 ? kUmmaKv4Threads : kUmmaAttnThreads;
-  constexpr size_t smem = 4 * 128 * 128 + static_cast<size_t>(STAGES) * 2 * (DH / 64) * 64 * 128 + (KV4 ? kv4_raw_bytes<DH>() : 0) + (2 * STAGES + 12) * 8 + 16 + 1024;
-  static_assert(smem <= 227 * 1024, "shared memory of one CTA");
+  constexpr size_t smem = Form::SMEM;
   static bool configured = false;
-  if (KV4 || !configured) {      // (the attribute belongs to a device: KV4 asks for it on whichever is the current one)
-    if (cudaFuncSetAttribute(attn_prompt_umma_kernel<DH, STAGES, KV4>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess) {
+  if (Form::KV4 || !configured) {      // (the attribute belongs to a device: KV4 asks for it on whichever is the current one)
+    if (cudaFuncSetAttribute(attn_prompt_umma_kernel<Form>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess) {
       set_error("attention_prompt_umma: cannot reserve %zu bytes of shared memory", smem);
       return kCudaError;
     }
     configured = true;
   }
-  static_assert(smem >= 256 * (DH + 4) * 4 + (2 * STAGES + 12) * 8 + 16 + 1024, "the sums of a CTA's rows");
   const dim3 grid(a.kv_heads, ceil_div(max_rows, a.cta_rows), n_seqs * a.splits);
   if (a.splits == 1) {
-    TIE_LAUNCH((attn_prompt_umma_kernel<DH, STAGES, KV4>), grid, THREADS, smem, s, km, vm, a);
+    TIE_LAUNCH((attn_prompt_umma_kernel<Form>), grid, Form::THREADS, smem, s, km, vm, a);
     return kOk;
   }
   // clusters of CTAs that hold tensor memory are not started beside the kernel ahead
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
-  cfg.blockDim = dim3(THREADS);
+  cfg.blockDim = dim3(Form::THREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr;
@@ -646,7 +709,7 @@ static int launch_prompt_umma(const CUtensorMap& km, const CUtensorMap& vm, cons
   attr.val.clusterDim.z = a.splits;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, attn_prompt_umma_kernel<DH, STAGES, KV4>, km, vm, a);
+  cudaLaunchKernelEx(&cfg, attn_prompt_umma_kernel<Form>, km, vm, a);
   return kOk;
 }
 
@@ -675,17 +738,18 @@ static void cut_prompt_umma(UmmaPromptArgs& a, int max_queries, int n_seqs, int 
 // of 512, 342, 172 and 2 tokens of 16 heads of 64 over 4 at 8,192 keys: one share 170, two 96, four 151 (the rule: two); 512 tokens of
 // 32 heads of 128 over 8 at 8,192 keys 184, 107, 135 (two); 128 tokens at 4,096 keys 98, 63, 47 (four); 1,024 tokens at 4,096 keys 100, 115, 176
 // (one); eight portions of 300 to 2 tokens at 4,096 keys 184, 176, 235 (two); 300 tokens at 300 keys 17.7, 22, 42, 128 rows 16.1 (128 rows).
-static void cut_prompt_kv4(UmmaPromptArgs& a, int max_queries, int n_seqs, int max_keys) {
+static void cut_prompt_kv4(UmmaPromptArgs& a, int row_tiles, int max_queries, int n_seqs, int max_keys) {
   const long long group = a.q_heads / a.kv_heads, max_rows = max_queries * group;
   const int keys = a.window > 0 && a.window + max_queries < max_keys ? a.window + max_queries : max_keys;
   const double tiles = (keys + kKeysPerTile - 1) / kKeysPerTile;
   double best = 0.0;
-  const int ways[4][3] = {{1, 256, 0}, {1, 128, 0}, {2, 256, 8}, {4, 256, 12}};
+  const int whole = 128 * row_tiles;      // (forms of one row tile a CTA: only shares)
+  const int ways[4][3] = {{1, whole, 0}, {1, 128, 0}, {2, whole, 8}, {4, whole, 12}};
   for (int i = 0; i < 4; ++i) {
     const int splits = ways[i][0], rows = ways[i][1];
     const long long most = n_seqs * ((max_rows + rows - 1) / rows), about = (2 * a.tokens * group + (n_seqs + 1) * rows) / (2 * rows);
     const long long ctas = a.kv_heads * (most < about ? most : about) * splits, places = splits == 4 ? 132 : 148;
-    const double cost = static_cast<double>((ctas + places - 1) / places) * (rows == 128 ? 0.86 : 1.0) * (tiles / splits + ways[i][2]);
+    const double cost = static_cast<double>((ctas + places - 1) / places) * (rows < whole ? 0.86 : 1.0) * (tiles / splits + ways[i][2]);
     if (i == 0 || cost < best) best = cost, a.splits = splits, a.cta_rows = rows;
   }
 }
@@ -723,21 +787,24 @@ TIE_API int tie_attention_prompt_umma(const void* q, long long q_stride, const v
                    status_word(), q_stride, max_blocks, q_heads, kv_heads, page_size, shift, window, scale * 1.4426950408889634f, 1, 256};
   const int max_rows = max_queries * (q_heads / kv_heads);
   cut_prompt_umma(a, max_queries, n_seqs, max_keys);
-  const int st = head_dim == 64 ? launch_prompt_umma<64, false>(km, vm, a, n_seqs, max_rows, s) : launch_prompt_umma<128, false>(km, vm, a, n_seqs, max_rows, s);
+  const int st = head_dim == 64 ? launch_prompt_umma<UmmaForm<64, false, 2, false>>(km, vm, a, n_seqs, max_rows, s)
+                                : launch_prompt_umma<UmmaForm<128, false, 2, false>>(km, vm, a, n_seqs, max_rows, s);
   if (st != kOk) return st;
   TIE_RETURN_LAUNCH("attention_prompt_umma");
 }
 
-// The same over a cache in 4 bits: heads of up to 128, a multiple of 8; pages of any size; q rows 16-byte aligned.
-TIE_API int tie_attention_prompt_kv4(const void* q, long long q_stride, long long tokens, const void* k_codes, const void* k_words, const void* v_codes,
-                                     const void* v_words, void* out, const int* query_start, const int* context_lens, const int* block_tables, int max_blocks,
-                                     int n_seqs, int max_queries, int q_heads, int kv_heads, int head_dim, int page_size, long long pages, int window, float scale,
-                                     int max_keys, cudaStream_t s) {
-  TIE_REQUIRE(head_dim > 0 && head_dim <= 128 && head_dim % 8 == 0, "attention_prompt_kv4: head_dim %d is not a multiple of 8 up to 128", head_dim);
+// The same over a cache in 4 bits: heads of a multiple of 8 up to 256 (float rows: 128); pages of any size; rows of q 16-byte aligned.
+TIE_API int tie_attention_prompt_kv4(int dtype, const void* q, long long q_stride, long long tokens, const void* k_codes, const void* k_words,
+                                     const void* v_codes, const void* v_words, void* out, const int* query_start, const int* context_lens,
+                                     const int* block_tables, int max_blocks, int n_seqs, int max_queries, int q_heads, int kv_heads, int head_dim, int page_size,
+                                     long long pages, int window, float scale, int max_keys, cudaStream_t s) {
+  const bool f32 = dtype == TIE_F32;
+  TIE_REQUIRE(head_dim > 0 && head_dim <= (f32 ? 128 : 256) && head_dim % 8 == 0, "attention_prompt_kv4: head_dim %d is not a multiple of 8 up to %d", head_dim,
+              f32 ? 128 : 256);
   TIE_REQUIRE(q_heads > 0 && kv_heads > 0 && q_heads % kv_heads == 0, "attention_prompt_kv4: %d query heads over %d kv heads", q_heads, kv_heads);
-  TIE_REQUIRE(q_stride % 8 == 0 && reinterpret_cast<uintptr_t>(q) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0,
+  TIE_REQUIRE(q_stride * (f32 ? 4 : 2) % 16 == 0 && reinterpret_cast<uintptr_t>(q) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0,
               "attention_prompt_kv4: q and out rows must be 16-byte aligned");
-  TIE_REQUIRE(page_size > 0 && pages > 0 && pages * page_size < (1LL << 31) && max_blocks >= 0 && n_seqs >= 0 && n_seqs <= 16383 && max_queries >= 0,
+  TIE_REQUIRE(page_size > 0 && pages > 0 && pages * page_size * kv_heads < (1LL << 31) && max_blocks >= 0 && n_seqs >= 0 && n_seqs <= 16383 && max_queries >= 0,
               "attention_prompt_kv4: bad sizes (%lld pages of %d, %d sequences, %d queries)", pages, page_size, n_seqs, max_queries);
   TIE_REQUIRE(scale > 0.0f, "attention_prompt_kv4: the scale must be positive");
   if (n_seqs == 0 || max_queries == 0) return kOk;
@@ -750,11 +817,17 @@ TIE_API int tie_attention_prompt_kv4(const void* q, long long q_stride, long lon
   UmmaPromptArgs a{static_cast<const __nv_bfloat16*>(q), static_cast<__nv_bfloat16*>(out), query_start, context_lens, block_tables, status_word(), q_stride, max_blocks,
                    q_heads, kv_heads, page_size, shift, window, scale * 1.4426950408889634f * kKv4Unscale, 1, 256, static_cast<const uint8_t*>(k_codes),
                    static_cast<const uint8_t*>(v_codes), static_cast<const uint16_t*>(k_words), static_cast<const uint16_t*>(v_words), head_dim,
-                   static_cast<int>(pages), tokens};
-  cut_prompt_kv4(a, max_queries, n_seqs, max_keys);
+                   static_cast<int>(pages), max_queries, tokens};
+  cut_prompt_kv4(a, f32 || head_dim > 128 ? 1 : 2, max_queries, n_seqs, max_keys);
   const CUtensorMap none = {};
-  const int st = head_dim <= 64 ? launch_prompt_umma<64, true>(none, none, a, n_seqs, static_cast<int>(all_rows), s)
-                                : launch_prompt_umma<128, true>(none, none, a, n_seqs, static_cast<int>(all_rows), s);
+  const int rows = static_cast<int>(all_rows);
+  int st;
+  if (f32) st = head_dim <= 64 ? launch_prompt_umma<UmmaForm<64, true, 1, true>>(none, none, a, n_seqs, rows, s)
+                               : launch_prompt_umma<UmmaForm<128, true, 1, true>>(none, none, a, n_seqs, rows, s);
+  else if (head_dim <= 64) st = launch_prompt_umma<UmmaForm<64, true, 2, false>>(none, none, a, n_seqs, rows, s);
+  else if (head_dim <= 128) st = launch_prompt_umma<UmmaForm<128, true, 2, false>>(none, none, a, n_seqs, rows, s);
+  else if (head_dim <= 192) st = launch_prompt_umma<UmmaForm<192, true, 1, false>>(none, none, a, n_seqs, rows, s);
+  else st = launch_prompt_umma<UmmaForm<256, true, 1, false>>(none, none, a, n_seqs, rows, s);
   if (st != kOk) return st;
   TIE_RETURN_LAUNCH("attention_prompt_kv4");
 }

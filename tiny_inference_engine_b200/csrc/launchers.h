@@ -79,7 +79,7 @@ TIE_API int tie_attention_kv4(int dtype, const void* q, long long q_stride, long
                               const void* v_words, void* out, const int* query_start, const int* context_lens, const int* block_tables, int max_blocks, int seqs,
                               int max_queries, int q_heads, int kv_heads, int head_dim, int page_size, long long pages, int window, float scale, const int* seq_list,
                               int n_list, int max_context, float* scratch, int* counters, cudaStream_t s);
-TIE_API int tie_attention_prompt_kv4(const void* q, long long q_stride, long long tokens, const void* k_codes, const void* k_words, const void* v_codes,
+TIE_API int tie_attention_prompt_kv4(int dtype, const void* q, long long q_stride, long long tokens, const void* k_codes, const void* k_words, const void* v_codes,
                                      const void* v_words, void* out, const int* query_start, const int* context_lens, const int* block_tables, int max_blocks,
                                      int n_seqs, int max_queries, int q_heads, int kv_heads, int head_dim, int page_size, long long pages, int window, float scale,
                                      int max_keys, cudaStream_t s);

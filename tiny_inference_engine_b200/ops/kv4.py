@@ -87,7 +87,13 @@ def _fail(msg: str):
     raise InvalidArgument(msg)
 
 
-UMMA_MIN_ROWS = 128     # rows (queries x heads of a group) from which the tcgen05 kernel takes a portion of a prompt
+# When the tcgen05 kernel takes the portions of a prompt, in place of the one whose warps take 16 rows each: from UMMA_MIN_ROWS rows (queries x heads
+# of a group) a portion, and UMMA_GROUPS of 16 rows in all, or with long contexts UMMA_FEW_GROUPS (groups x keys UMMA_GROUPS x 1,024). It starts
+# slower (9 to 15 us a call against 5 to 10) and its tiles of 128 rows are too few for the GPU until then. bfloat16, 32 heads over 8 of 128, us with
+# it and without: 64 portions of 16 rows at 512 keys 69 and 26, 32 of 48 rows at 64 18 and 21, 16 of 64 rows 10 and 15; one of 64 queries at 300 keys (128
+# groups) 18 and 10, 128 at 1,024 (256 groups) 29 and 20, at 2,048 35 and 44, 192 at 1,024 (384 groups) 29 and 33, 512 at 512 20 and 38; 4
+# of 512 at 2,048 105 and 396. float32: 64 at 300 20 and 11, 192 at 1,024 35 and 44, 4 of 512 at 2,048 205 and 646.
+UMMA_MIN_ROWS, UMMA_GROUPS, UMMA_FEW_GROUPS = 48, 384, 128
 _FLOATS = {torch.float32: 0, torch.bfloat16: 1}
 _I32 = torch.int32
 
@@ -254,23 +260,30 @@ def attention_kv4_decode(q, cache: Kv4Cache, out, query_start, context_lens, blo
         _rows_kernel(checked, q, out, query_start, context_lens, block_tables, 1, q_heads, scale, window, seq_list.data_ptr(), n_list, max_context, workspace)
 
 
+def _on_tcgen05(dtype, sizes, T, group, n_seqs, max_queries, keys):
+    rows, head_dim = max_queries * group, sizes[1]
+    if rows < UMMA_MIN_ROWS or head_dim > (256 if dtype else 128) or head_dim % 8 or n_seqs > 16383 or rows > 65535 * 128:
+        return False
+    groups = sizes[0] * min(n_seqs * ((rows + 15) // 16), T * group // 16 + n_seqs)
+    return groups >= UMMA_GROUPS or (groups >= UMMA_FEW_GROUPS and groups * keys >= UMMA_GROUPS * 1024)
+
+
 def attention_kv4_prompt(q, cache: Kv4Cache, out, query_start, context_lens, block_tables, n_seqs: int, max_queries: int, q_heads: int, scale: float,
                          max_context: int, workspace: Kv4Workspace, window: int = 0) -> None:
     """Causal attention of the first n_seqs sequences of the step, each bringing up to max_queries tokens that are in the cache already: row t of
     sequence s sits at pos = context_lens[s] - (its queries) + (t - query_start[s]) and sees keys 0..pos (with a window: the last `window` of
     them). A sequence that brings more than max_queries tokens has its first ones only, the other rows are left as they are. Types, layouts and
-    `max_context` as in `attention_kv4_decode`; bfloat16 rows of long portions (UMMA_MIN_ROWS, heads of up to 128, a multiple of 8) run on
-    tcgen05, where weights enter the value product as one bfloat16 number."""
+    `max_context` as in `attention_kv4_decode`; long portions (`UMMA_MIN_ROWS` and what stands there; 16-byte aligned rows, heads of a multiple of 8
+    up to 256, float32 128) run on tcgen05, where the weights of bfloat16 rows enter the value product as one bfloat16 number."""
     checked = _check_attention("attention_kv4_prompt", q, cache, out, query_start, context_lens, block_tables, q_heads, workspace, window, n_seqs, scale,
                                max_context, max_queries)
     max_queries = min(max_queries, checked[3])
     if not n_seqs or not max_queries:
         return
     dtype, planes, sizes, T, q_stride, _, columns, stream = checked
-    rows = max_queries * (q_heads // sizes[0])
-    if dtype == 1 and rows >= UMMA_MIN_ROWS and sizes[1] <= 128 and sizes[1] % 8 == 0 and q_stride % 8 == 0 and not (q.data_ptr() | out.data_ptr()) & 15 and \
-            n_seqs <= 16383 and rows <= 65535 * 128:
-        call("tie_attention_prompt_kv4", q.data_ptr(), q_stride, T, *planes, out.data_ptr(), query_start.data_ptr(), context_lens.data_ptr(),
+    if _on_tcgen05(dtype, sizes, T, q_heads // sizes[0], n_seqs, max_queries, min(max_context, window + max_queries) if window else max_context) and \
+            q_stride % (8 if dtype else 4) == 0 and not (q.data_ptr() | out.data_ptr()) & 15:
+        call("tie_attention_prompt_kv4", dtype, q.data_ptr(), q_stride, T, *planes, out.data_ptr(), query_start.data_ptr(), context_lens.data_ptr(),
              block_tables.data_ptr(), columns, n_seqs, max_queries, q_heads, *sizes, window, scale, min(max_context, 2 ** 30), stream)
     else:
         _rows_kernel(checked, q, out, query_start, context_lens, block_tables, max_queries, q_heads, scale, window, 0, n_seqs, max_context, workspace)

@@ -120,7 +120,7 @@ _SIGNATURES = {
     "tie_kv4_append": [I, P, P, L, L, P, P, P, P, P, I, I, I, I, L, P],
     "tie_kv4_read": [I, P, P, P, P, P, P, P, L, L, I, I, I, I, L, P],
     "tie_attention_kv4": [I, P, L, L, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, L, I, F, P, I, I, P, P, P],
-    "tie_attention_prompt_kv4": [P, L, L, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, L, I, F, I, P],
+    "tie_attention_prompt_kv4": [I, P, L, L, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, L, I, F, I, P],
     "tie_step_tables": [P] * 14 + [I] * 8 + [P],
     "tie_release_tables": [P] * 6 + [I] * 5 + [P],
     "tie_attention_mixed": [I, P, L, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, F, I, P, I, I, I, P, P],
