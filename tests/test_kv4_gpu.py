@@ -88,6 +88,25 @@ def test_append_and_read(dtype, T, kv_heads, head_dim, page, strided):
     assert (err <= np.repeat(s, 32, -1)[..., :head_dim] * 1.0000001 + 2.0 ** -100).all()
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("step", [1.0, 1.25, 1.75 * 2.0 ** 40, 2.0 ** -90])
+def test_append_of_halves_that_round_up_at_both_ends(dtype, step):
+    """The least -7.5 steps, the largest 7.5: z is 8 and the largest would be code 16. Halves and steps between them, in every place of a group."""
+    rng = np.random.default_rng(3)
+    x = (rng.integers(-15, 16, (64, 2, 80)) / 2 * step).astype(np.float32)
+    for t in range(64):
+        x[t, :, t % 32::32] = 7.5 * step
+        x[t, :, (t + 1 + t // 32) % 32::32] = -7.5 * step
+    cache = ops.kv4_cache(4, 2, 16, 80)
+    ops.kv4_append(cuda(x.reshape(64, -1), DT[dtype]), cuda(-x.reshape(64, -1), DT[dtype]), cuda(np.arange(64)), cache)
+    (kc, kw), (vc, vw) = plain.quantise(x, -x)
+    order = lambda t: t.cpu().numpy().transpose(0, 2, 1, 3).reshape(64, 2, -1)
+    assert np.array_equal(order(cache.k_codes), kc) and np.array_equal(order(cache.v_codes), vc)
+    assert np.array_equal(order(cache.k_words), kw) and np.array_equal(order(cache.v_words), vw)
+    top = np.stack([kc & 15, kc >> 4], -1).reshape(64, 2, -1)
+    assert (top[np.arange(64), :, np.arange(64) % 32] == 15).all()
+
+
 def test_append_marks_numbers_that_are_not_finite():
     T, heads, dim, page = 6, 2, 96, 4
     rng = np.random.default_rng(0)

@@ -1,14 +1,17 @@
 // Keys and values into a cache in 4 bits (the format: kv4.cuh), and out of it again.
 //
 // Both move memory: a token and head has 4 head_dim bytes of bfloat16 keys and values on one side and 9/8 head_dim bytes of codes and words on
-// the other. Eight dimensions (one 32-bit word of codes, 16 bytes of bfloat16) are one thread's; four threads share a group and meet in two
-// shuffles; a token and head is one warp (half of one up to 64 dimensions), which also settles by one vote whether all its numbers are finite.
+// the other. 8,192 tokens of 8 heads of 128 in bfloat16: in 10.3 us, out 10.0 us (38 MB each; 33 MB filled with zeros take 9.5 us, copied from
+// L2 6.8 us). What is stored is bound by instructions: with 8 dimensions a thread, whose group's step, its reciprocal and the places of what is stored
+// were worked out four times instead of twice, 14.8 us; with one float at a time instead of two 16.3 us.
 #include "kv4.cuh"
 #include "launchers.h"
 
 namespace tie {
 
 int* status_word();
+
+constexpr int kKv4Blocks = 65535;        // of a head, before blockIdx.z counts on
 
 struct Kv4Planes {
   uint32_t *k_codes, *v_codes;
@@ -23,15 +26,12 @@ __device__ __forceinline__ int kv4_row(int slot, int head, const Kv4Planes& c) {
   return (page * c.kv_heads + head - page) * c.page_size + slot;
 }
 
-// A head's token: up to two 64s (NG) its key and value are the lanes of a warp side by side (one 64: of half a warp), else every lane has a word
-// of both. blockIdx.y is the head, the block's warps (halves) take tokens in turn.
+// Where a thread of kv4_append works: 16 dimensions (half a group) of a token's key or value of one head. The lanes of a token and head, its key's first, lie side by
+// side in a warp; blockIdx.x is the head, the block's tokens come in turn.
 template <int NG> struct Kv4Lanes {
-  static constexpr int W = 8 * NG;                        // words of codes of a head
-  static constexpr int ITEMS = NG <= 2 ? 1 : 2;           // words of a lane
-  static constexpr int LANES = NG == 1 ? 16 : 32;
-  static constexpr int STEP = 256 / LANES;                // tokens that a block has at a time
-  static __device__ __forceinline__ bool is_value(int lane, int item) { return ITEMS == 2 ? item == 1 : lane >= W; }
-  static __device__ __forceinline__ int word(int lane) { return ITEMS == 2 ? lane : lane % W; }
+  static constexpr int PLANE = 4 * NG;                                 // lanes of a key, or of a value
+  static constexpr int LANES = NG == 1 ? 8 : NG == 2 ? 16 : 32;        // (heads of three 64s leave eight idle)
+  static constexpr int STEP = 256 / LANES;                             // tokens that a block has at a time
 };
 
 // Adding it rounds a float below 2^22 to a whole number, ties to even, and leaves that number in the low bits.
@@ -44,15 +44,58 @@ __device__ __forceinline__ float kv4_quotient(float x, float s, float reciprocal
   const float q = x * reciprocal;
   return __fadd_rn(__fadd_rn(fmaf(fmaf(-q, s, x), reciprocal, q), kRoundMagic), add - kRoundMagic);
 }
-__device__ __forceinline__ float max_nan(float a, float b) {
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
   float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-__device__ __forceinline__ float min_nan(float a, float b) {
+__device__ __forceinline__ float min_nan(float a, float b, float c) {
   float d;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
+}
+
+// Two floats that sm_100a works on as one.
+using Pair = unsigned long long;
+__device__ __forceinline__ Pair pair(float a, float b) {
+  Pair d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ Pair fma_pair(Pair a, Pair b, Pair c) {
+  Pair d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ Pair mul_pair(Pair a, Pair b) {
+  Pair d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ Pair add_pair(Pair a, Pair b) {
+  Pair d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+// Eight values as codes. Four codes are the digits of one number, whose bits 2^23 shows; dimensions 0-3 and 4-7 side by side.
+// rint(x / s) >= rint(lo / s) = -z, and rint(x / s) + z is above 15 only where both x / s and -lo / s are halves that round up, and then
+// 16: `top` says so for the group.
+__device__ __forceinline__ uint32_t kv4_codes(const float* x, float s, float reciprocal, float z, bool top) {
+  if (!top) {
+    const Pair s2 = pair(-s, -s), r2 = pair(reciprocal, reciprocal), magic = pair(kRoundMagic, kRoundMagic), back = pair(z - kRoundMagic, z - kRoundMagic);
+    Pair four = pair(128.0f, 128.0f);       // 2^23 when four digits have come in
+#pragma unroll
+    for (int e = 3; e >= 0; --e) {
+      const Pair v2 = pair(x[e], x[4 + e]), q = mul_pair(v2, r2);
+      four = fma_pair(four, pair(16.0f, 16.0f), add_pair(add_pair(fma_pair(fma_pair(q, s2, v2), r2, q), magic), back));
+    }
+    return __byte_perm(static_cast<uint32_t>(four), static_cast<uint32_t>(four >> 32), 0x5410);
+  }
+  uint32_t codes = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) codes |= (__float_as_uint(fminf(kv4_quotient(x[e], s, reciprocal, z), 15.0f) + 8388608.0f) & 15u) << (4 * e);
+  return codes;
 }
 
 // ROUNDS: tokens that a thread takes one after the other, and works out its place in a head for once.
@@ -61,74 +104,68 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const T* __restrict__ k
                                                          const int* __restrict__ slots, Kv4Planes c, int tokens, int vec, int* status) {
   pdl_sync();
   using L = Kv4Lanes<NG>;
-  const int lane = threadIdx.x & (L::LANES - 1), head = blockIdx.y, word = L::word(lane);
-  const uint32_t mine = NG == 1 ? 0xffffu << (threadIdx.x & 16) : 0xffffffffu;
-  const int dims = word < L::W ? c.head_dim - word * 8 : 0;
-  const T* src[L::ITEMS];
-  long long stride[L::ITEMS];
-#pragma unroll
-  for (int i = 0; i < L::ITEMS; ++i) {
-    src[i] = (L::is_value(lane, i) ? v : k) + static_cast<long long>(head) * c.head_dim + word * 8;
-    stride[i] = L::is_value(lane, i) ? v_stride : k_stride;
-  }
-#pragma unroll 2
+  const int lane = threadIdx.x & (L::LANES - 1), head = blockIdx.x, is_v = lane >= L::PLANE, part = lane - (is_v ? L::PLANE : 0);
+  const uint32_t mine = L::LANES == 32 ? 0xffffffffu : ((1u << (L::LANES & 31)) - 1u) << (threadIdx.x & (32 - L::LANES));
+  const int dims = part < L::PLANE ? c.head_dim - part * 16 : 0;
+  const long long stride = is_v ? v_stride : k_stride;
+  const int first = (blockIdx.z * kKv4Blocks + blockIdx.y) * (ROUNDS * L::STEP) + threadIdx.x / L::LANES;
+  const T* src = (is_v ? v : k) + static_cast<long long>(head) * c.head_dim + part * 16 + first * stride;
+  uint32_t* const codes = is_v ? c.v_codes : c.k_codes;
+  uint16_t* const words = is_v ? c.v_words : c.k_words;
+#pragma unroll 1          // (2: 32,768 tokens 49 us instead of 43)
   for (int round = 0; round < ROUNDS; ++round) {
-    const int token = blockIdx.x * (ROUNDS * L::STEP) + round * L::STEP + threadIdx.x / L::LANES;
+    const int token = first + round * L::STEP;
     const int slot = token < tokens ? slots[token] : -1;
     const bool writes = slot >= 0 && static_cast<unsigned int>(slot) < c.slots;
     if (slot >= 0 && !writes && lane == 0) *reinterpret_cast<volatile int*>(status) = kStatusBadSlot;
-    float x[L::ITEMS][8], lo[L::ITEMS], hi[L::ITEMS];
-    bool fine = true;
+    float x[16];
+    load8(src + round * L::STEP * stride, writes ? dims : 0, vec != 0, reinterpret_cast<float(&)[8]>(x[0]));
+    load8(src + round * L::STEP * stride + 8, writes ? dims - 8 : 0, vec != 0, reinterpret_cast<float(&)[8]>(x[8]));
+    float lo = 0.0f, hi = 0.0f;
 #pragma unroll
-    for (int i = 0; i < L::ITEMS; ++i) {
-      load8(src[i] + token * stride[i], writes ? dims : 0, vec != 0, x[i]);
-      lo[i] = hi[i] = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) lo[i] = min_nan(lo[i], x[i][e]), hi[i] = max_nan(hi[i], x[i][e]);
-      fine = fine && hi[i] < kKv4Limit && lo[i] > -kKv4Limit;      // (false for NaN)
+    for (int e = 0; e < 16; e += 2) lo = min_nan(lo, x[e], x[e + 1]), hi = max_nan(hi, x[e], x[e + 1]);
+    const bool fine = (__ballot_sync(0xffffffffu, hi < kKv4Limit && lo > -kKv4Limit) & mine) == mine;      // (false for NaN)
+    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, 1));
+    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, 1));
+    uint2 out = make_uint2(0u, 0u);
+    uint32_t w = is_v ? 0u : kKv4NaN;
+    if (fine) {
+      const float s = kv4_step(lo, hi), reciprocal = __frcp_rn(s);
+      const float z = kv4_quotient(-lo, s, reciprocal, 0.0f);
+      const bool top = kv4_quotient(hi, s, reciprocal, z) > 15.0f;
+      out = make_uint2(kv4_codes(x, s, reciprocal, z, top), kv4_codes(x + 8, s, reciprocal, z, top));
+      w = (__float_as_uint(s) >> 16) | (__float_as_uint(z + 8388608.0f) & 15u);
     }
-    fine = (__ballot_sync(0xffffffffu, fine) & mine) == mine;
-    const int at = kv4_row(writes ? slot : 0, head, c);
-#pragma unroll
-    for (int i = 0; i < L::ITEMS; ++i) {
-      const bool is_v = L::is_value(lane, i);
-#pragma unroll
-      for (int o = 1; o <= 2; o <<= 1) {
-        lo[i] = fminf(lo[i], __shfl_xor_sync(0xffffffffu, lo[i], o));
-        hi[i] = fmaxf(hi[i], __shfl_xor_sync(0xffffffffu, hi[i], o));
-      }
-      uint32_t codes = 0, w = is_v ? 0u : kKv4NaN;
-      if (fine) {
-        const float s = kv4_step(lo[i], hi[i]), reciprocal = __frcp_rn(s);
-        const float z = kv4_quotient(-lo[i], s, reciprocal, 0.0f);
-        // four codes as the digits of one number, whose bits 2^23 shows. (rint(x / s) >= rint(lo / s) = -z: only the upper end is to be clamped)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float four = 0.0f;
-#pragma unroll
-          for (int e = 3; e >= 0; --e) four = fmaf(four, 16.0f, fminf(kv4_quotient(x[i][4 * h + e], s, reciprocal, z), 15.0f));
-          codes |= (__float_as_uint(four + 8388608.0f) & 0xffffu) << (16 * h);
-        }
-        w = (__float_as_uint(s) >> 16) | (__float_as_uint(z + 8388608.0f) & 15u);
-      }
-      if (writes && word < L::W) {
-        (is_v ? c.v_codes : c.k_codes)[static_cast<long long>(at) * L::W + word] = codes;
-        if ((word & 3) == 0) (is_v ? c.v_words : c.k_words)[static_cast<long long>(at) * (L::W / 4) + word / 4] = static_cast<uint16_t>(w);
-      }
+    if (writes && part < L::PLANE) {
+      const long long at = static_cast<long long>(kv4_row(slot, head, c)) * L::PLANE + part;
+      reinterpret_cast<uint2*>(codes)[at] = out;
+      if ((part & 1) == 0) words[at >> 1] = static_cast<uint16_t>(w);
     }
   }
 }
+
+// Where a thread of kv4_read works: 8 dimensions, so that neighbours write 16 bytes side by side (with 16 dimensions 2,049 tokens of 5 heads of 96 in
+// float 4.8 us instead of 3.5). A head's token: up to two 64s its key and value are the lanes of a warp (one 64: of half a warp), else every lane has
+// a word of both. blockIdx.x is the head, the block's warps (halves) take tokens in turn.
+template <int NG> struct Kv4ReadLanes {
+  static constexpr int W = 8 * NG;                        // words of codes of a head
+  static constexpr int ITEMS = NG <= 2 ? 1 : 2;           // words of a lane
+  static constexpr int LANES = NG == 1 ? 16 : 32;
+  static constexpr int STEP = 256 / LANES;                // tokens that a block has at a time
+  static __device__ __forceinline__ bool is_value(int lane, int item) { return ITEMS == 2 ? item == 1 : lane >= W; }
+  static __device__ __forceinline__ int word(int lane) { return ITEMS == 2 ? lane : lane % W; }
+};
 
 template <typename T, int NG, int ROUNDS>
 __global__ void __launch_bounds__(256) kv4_read_kernel(Kv4Planes c, const int* __restrict__ slots, T* __restrict__ k, T* __restrict__ v, long long k_stride,
                                                        long long v_stride, int tokens, int vec, int* status) {
   pdl_sync();
-  using L = Kv4Lanes<NG>;
-  const int lane = threadIdx.x & (L::LANES - 1), head = blockIdx.y, word = L::word(lane), left = c.head_dim - word * 8;
+  using L = Kv4ReadLanes<NG>;
+  const int lane = threadIdx.x & (L::LANES - 1), head = blockIdx.x, word = L::word(lane), left = c.head_dim - word * 8;
   if (word >= L::W || left <= 0) return;
 #pragma unroll 4
   for (int round = 0; round < ROUNDS; ++round) {
-    const int token = blockIdx.x * (ROUNDS * L::STEP) + round * L::STEP + threadIdx.x / L::LANES;
+    const int token = (blockIdx.z * kKv4Blocks + blockIdx.y) * (ROUNDS * L::STEP) + round * L::STEP + threadIdx.x / L::LANES;
     const int slot = token < tokens ? slots[token] : -1;
     if (slot < 0) continue;
     if (static_cast<unsigned int>(slot) >= c.slots) {
@@ -173,16 +210,18 @@ static bool kv4_rows_aligned(const void* k, const void* v, long long k_stride, l
 template <typename T, int NG, int ROUNDS>
 static void launch_kv4(bool append, T* k, T* v, long long k_stride, long long v_stride, const int* slots, const Kv4Planes& c, int tokens, cudaStream_t s) {
   const int vec = kv4_rows_aligned(k, v, k_stride, v_stride, c.head_dim, sizeof(T)) ? 1 : 0;
-  const dim3 grid(ceil_div(tokens, ROUNDS * Kv4Lanes<NG>::STEP), c.kv_heads);
+  const int blocks = ceil_div(tokens, ROUNDS * (append ? Kv4Lanes<NG>::STEP : Kv4ReadLanes<NG>::STEP));
+  const dim3 grid(c.kv_heads, min(blocks, kKv4Blocks), ceil_div(blocks, kKv4Blocks));
   if (append) TIE_LAUNCH((kv4_append_kernel<T, NG, ROUNDS>), grid, 256, 0, s, k, v, k_stride, v_stride, slots, c, tokens, vec, status_word());
   else TIE_LAUNCH((kv4_read_kernel<T, NG, ROUNDS>), grid, 256, 0, s, c, slots, k, v, k_stride, v_stride, tokens, vec, status_word());
 }
 
-// Four tokens a thread where that still leaves every SM eight blocks: 8,192 tokens of 8 heads of 128 in and out 28 us against 30 with one; but
-// 2,049 of 5 heads of 96 11.1 against 8.8, eight tokens 4.8 against 3.3.
+// Four tokens a thread where that still leaves every SM eight blocks. (One token: 8,192 of 8 heads of 128 in and out 2 us more; four everywhere: 2,049
+// of 5 heads of 96 11.1 us instead of 8.8, eight tokens 4.8 instead of 3.3.)
 template <typename T, int NG>
 static void launch_kv4(bool append, T* k, T* v, long long k_stride, long long v_stride, const int* slots, const Kv4Planes& c, int tokens, cudaStream_t s) {
-  if (static_cast<long long>(tokens / (4 * Kv4Lanes<NG>::STEP)) * c.kv_heads >= 148 * 8) launch_kv4<T, NG, 4>(append, k, v, k_stride, v_stride, slots, c, tokens, s);
+  const int blocks = tokens / (4 * (append ? Kv4Lanes<NG>::STEP : Kv4ReadLanes<NG>::STEP));
+  if (static_cast<long long>(blocks) * c.kv_heads >= 148 * 8) launch_kv4<T, NG, 4>(append, k, v, k_stride, v_stride, slots, c, tokens, s);
   else launch_kv4<T, NG, 1>(append, k, v, k_stride, v_stride, slots, c, tokens, s);
 }
 
@@ -207,7 +246,7 @@ static Kv4Planes kv4_planes(const void* k_codes, const void* k_words, const void
 
 static int launch_kv4(const char* name, bool append, int dtype, const Kv4Planes& c, void* k, void* v, long long k_stride, long long v_stride, const int* slots, int tokens,
                       long long pages, cudaStream_t s) {
-  TIE_REQUIRE(tokens >= 0 && c.kv_heads > 0 && c.kv_heads <= 65535 && c.page_size > 0 && c.head_dim > 0 && c.head_dim <= 256,
+  TIE_REQUIRE(tokens >= 0 && tokens <= (1 << 30) && c.kv_heads > 0 && c.kv_heads <= 65535 && c.page_size > 0 && c.head_dim > 0 && c.head_dim <= 256,
               "%s: bad sizes (tokens %d, kv heads %d, page size %d, head size %d)", name, tokens, c.kv_heads, c.page_size, c.head_dim);
   TIE_REQUIRE(pages > 0 && pages * c.page_size < (1LL << 31), "%s: %lld pages of %d tokens: slots are 32-bit numbers", name, pages, c.page_size);
   TIE_REQUIRE(pages * c.page_size * c.kv_heads < (1LL << 31), "%s: planes of %lld x %d x %d rows: rows are 32-bit numbers", name, pages, c.kv_heads, c.page_size);
