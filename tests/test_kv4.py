@@ -60,6 +60,7 @@ def test_append_and_read_refuse(fn):
     refused(go, x, x.bfloat16(), s, cache(), match="alike")
     refused(go, x[:, :64], x[:, :64], s, cache())
     refused(go, x, x[:2], s, cache())
+    refused(go, x[:1].expand(3, -1), x, s, cache(), match="overlap" if fn == "read" else "CUDA")      # (append only reads them)
     refused(go, torch.zeros(3, 256)[:, ::2], x, s, cache())
     refused(go, x, x, s[:2], cache(), match="slots")
     refused(go, x, x, s.long(), cache(), match="slots")

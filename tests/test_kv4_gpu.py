@@ -289,6 +289,19 @@ def test_long_portions(monkeypatch, forced, dtype, window, contexts, queries, he
 
 
 @pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("window,head_dim", [(0, 64), (16, 128), (0, 192)])
+def test_long_portions_with_fewer_keys_than_queries_and_any_hint(monkeypatch, dtype, window, head_dim):
+    monkeypatch.setattr(kv4, "UMMA_GROUPS", 0)
+    b = Batch(6, [20, 0, 300, 129], [150, 140, 100, 129], 8, 2, head_dim, 16, dtype, window, pad=8)
+    for hint in (300, 1, 2 ** 31 - 1):       # how the launch is cut, not what it computes
+        b.out.fill_(9.0)
+        ops.attention_kv4_prompt(b.qt, b.cache, b.out, *b.args, 4, 150, b.heads, b.scale, hint, b.work, window=window)
+        got = b.answer()
+        b.check(got, one_term=True, truncated=True)
+        assert (got[:130] == 0.0).all() and (got[150:290] == 0.0).all()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
 @pytest.mark.parametrize("head_dim", [64, 128, 256])
 def test_long_portions_leave_the_rows_that_are_not_theirs(monkeypatch, dtype, head_dim):
     monkeypatch.setattr(kv4, "UMMA_GROUPS", 0)
@@ -367,6 +380,25 @@ def test_other_streams_and_graphs():
     b.out.fill_(0.0)
     graph.replay()
     assert np.array_equal(want, b.answer())
+
+
+def test_calls_at_the_same_time_with_workspaces_of_their_own():
+    batches = [Batch(20 + i, [4000, 300, 2500], [1] * 3, 8, 2, 128, 16, "bfloat16") for i in range(2)]
+    want = [b.decode() for b in batches]
+    streams, seqs = [torch.cuda.Stream() for _ in batches], cuda([0, 1, 2])
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for b, stream in zip(batches, streams):
+            with torch.cuda.stream(stream):
+                b.out.fill_(9.0)
+                ops.attention_kv4_decode(b.qt, b.cache, b.out, *b.args, b.heads, b.scale, seqs, 3, 4000, b.work)
+    for b, w in zip(batches, want):
+        assert np.array_equal(b.answer(), w)
+
+
+def test_a_sequence_that_is_listed_twice():
+    b = Batch(31, [5000, 70], [1, 1], 8, 2, 128, 16, "bfloat16")
+    b.check(b.decode(seqs=[0, 1, 0]))
 
 
 # ---- step tables

@@ -144,7 +144,7 @@ def _check_cache(what: str, c: Kv4Cache) -> tuple:
     return planes, (heads, dim, size, pages)
 
 
-def _check_rows(what: str, c: Kv4Cache, k, v, slots) -> tuple:
+def _check_rows(what: str, c: Kv4Cache, k, v, slots, written=False) -> tuple:
     planes, sizes = _check_cache(what, c)
     dtype = _FLOATS.get(k.dtype)
     if dtype is None or v.dtype is not k.dtype:
@@ -155,6 +155,8 @@ def _check_rows(what: str, c: Kv4Cache, k, v, slots) -> tuple:
     (k_stride, k_step), (v_stride, v_step) = k.stride(), v.stride()
     if (k_step != 1 or v_step != 1) and width > 1:
         _fail(f"{what}: k and v must be [T, {width}] with contiguous rows")
+    if written and shape[0] > 1 and (k_stride < width or v_stride < width):
+        _fail(f"{what}: rows of k and v must not overlap")
     if slots.dtype is not _I32 or slots.numel() != shape[0] or not slots.is_contiguous():
         _fail(f"{what}: slots must be contiguous int32 [{shape[0]}]")
     return dtype, planes, sizes, shape[0], k_stride, v_stride, _stream(what, k, v, slots, c[0], c[1], c[2], c[3])
@@ -170,8 +172,8 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: Kv4
 
 def kv4_read(cache: Kv4Cache, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
     """The values that the cache holds at slots[t] into k, v [T, kv_heads * head_dim] (float32 or bfloat16, exact in both); rows whose slot is below
-    zero are left as they are."""
-    dtype, planes, sizes, T, k_stride, v_stride, stream = _check_rows("kv4_read", cache, k, v, slots)
+    zero are left as they are. Rows of one tensor must not overlap."""
+    dtype, planes, sizes, T, k_stride, v_stride, stream = _check_rows("kv4_read", cache, k, v, slots, True)
     call("tie_kv4_read", dtype, *planes, slots.data_ptr(), k.data_ptr(), v.data_ptr(), k_stride, v_stride, T, *sizes, stream)
 
 
