@@ -33,8 +33,8 @@
 // Warps take the place of the TMA producer: they read codes and words some tiles ahead, take them apart and write the
 // tile as TMA would have. Heads above 128 leave tensor memory for one row tile a CTA; so do float queries, which
 // stand there as three bfloat16 terms (24 bits), as the weights do in shared memory. 4 portions of 512 queries at 2,048 keys, 32 heads over 8,
-// us against the kernel whose warps take 16 rows each: heads of 128 105 and 396 (float 205 and 646), of 64 92 and 267 (162 and 407), of 192
-// 203 and 589, of 256 330 and 790. Eight dimensions lie in a tile in the order 0 4 1 5 2 6 3 7, in which a word of codes comes apart; Q is put into tensor
+// us against the kernel whose warps take 16 rows each: heads of 128 98 and 396 (float 195 and 646), of 64 87 and 267 (162 and 407), of 192
+// 159 and 589, of 256 210 and 790. Eight dimensions lie in a tile in the order 0 4 1 5 2 6 3 7, in which a word of codes comes apart; Q is put into tensor
 // memory in the same order and the outputs are taken out of it again. Keys and values are exact in bfloat16, times 2^-64 (kv4.cuh).
 #include "attention_mma.cuh"
 #include "kv4.cuh"
@@ -89,15 +89,19 @@ struct UmmaForm {
   static constexpr int THREADS = !KV4 ? 320 : RT == 2 ? 384 : 352;
   static constexpr int PRODUCERS = RT == 2 ? 96 : 192;            // threads that take a KV4 tile apart
   static constexpr int STAGES = DH <= 64 ? (F32 ? 4 : 6) : DH == 128 ? (KV4 ? 3 : 4) : DH == 192 ? 3 : 2;
-  static constexpr int AHEAD = RT == 2 ? 3 : 2;                   // tiles that a producer copies ahead
+  static constexpr int AHEAD = 2;                                   // tiles that a producer copies ahead (3: heads of 64 88.6 us instead of 87.3, the others alike)
   static constexpr int ROUNDS = (kKeysPerTile * DH / 32 + PRODUCERS - 1) / PRODUCERS;     // keys (and values) of a producer thread in a tile
   static constexpr int RAW = ROUNDS * PRODUCERS * 40;             // bytes of a tile on its way: a thread's two times 16 bytes of codes and two words
+  // Pairs of barriers a stage: 1 for keys and values together; 2 with one for the keys, which are filled again while the values are still read. That
+  // pays where the producers are what the others wait for (4 portions of 512 queries at 2,048 keys, 32 heads over 8 of 256: 210 us instead of
+  // 235, of 64: 87 instead of 91) and else costs waits (of 128: 109 instead of 98; of 192: 174 instead of 159).
+  static constexpr int RINGS = KV4_ && !F32_ && (DH <= 64 || DH == 256) ? 2 : 1;
   static constexpr int P_BYTES = 128 * 128;                       // 128 rows x 64 keys
   static constexpr int STAGE_BYTES = 2 * (DH / 64) * 64 * 128;    // keys and values of a tile
   static constexpr int P_ALL = RT * 2 * TERMS * P_BYTES;          // [row tile][buffer][term]
-  static constexpr int SMEM = P_ALL + STAGES * STAGE_BYTES + (KV4 ? AHEAD * RAW : 0) + (2 * STAGES + 12) * 8 + 16 + 1024;
+  static constexpr int SMEM = P_ALL + STAGES * STAGE_BYTES + (KV4 ? AHEAD * RAW : 0) + (2 * RINGS * STAGES + 12) * 8 + 16 + 1024;
   static_assert(SMEM <= 227 * 1024, "shared memory of one CTA");
-  static_assert(SMEM >= RT * 128 * (DH + 4) * 4 + (2 * STAGES + 12) * 8 + 16 + 1024, "the sums of a CTA's rows");
+  static_assert(SMEM >= RT * 128 * (DH + 4) * 4 + (2 * RINGS * STAGES + 12) * 8 + 16 + 1024, "the sums of a CTA's rows");
 };
 
 // What the producer warps of a CTA do (KV4); `id` numbers their threads. A thread takes 32 dimensions (16 bytes of codes, one group) of
@@ -107,9 +111,11 @@ template <typename Form>
 __device__ __forceinline__ void kv4_produce(const UmmaPromptArgs& a, uint8_t* ring, uint8_t* raw, uint64_t* kv_full, uint64_t* kv_empty, volatile int* abort_flag,
                                             int id, int seq, int kvh, int kt_first, int n_tiles, int lo, int hi) {
   constexpr int GROUPS = Form::DH / 32, PER = Form::ROUNDS, RAW = Form::RAW, STAGES = Form::STAGES, PLANE_BYTES = Form::STAGE_BYTES / 2;
-  static_assert(Form::PRODUCERS % GROUPS == 0, "a thread's keys have one group");
-  const int group = id % GROUPS, first = id / GROUPS;            // keys first + j * STEP of a tile, below its 64
-  constexpr int STEP = Form::PRODUCERS / GROUPS;
+  static_assert(Form::PRODUCERS % (4 * GROUPS) == 0, "a thread's keys have one group");
+  // Eight threads have four keys' 64 dimensions: what they store at a time lies in eight different places of a row of 128 bytes. (With a key's groups
+  // side by side it lies in two to four: heads of 256 330 us instead of 235, of 192 203 instead of 159, of 128 105 instead of 98, as above.)
+  const int group = (id >> 3) % (GROUPS / 2) * 2 + (id & 1), first = (id >> 3) / (GROUPS / 2) * 4 + ((id >> 1) & 3);
+  constexpr int STEP = Form::PRODUCERS / GROUPS;                  // its keys: first + j * STEP of a tile, below its 64
   const int* table = a.block_tables + static_cast<long long>(seq) * a.max_blocks;
   const uint32_t signs = kv4_signs();
   int rows[PER];                  // of the tile that is copied next; what no row sees is row 0, and masked below
@@ -132,9 +138,9 @@ __device__ __forceinline__ void kv4_produce(const UmmaPromptArgs& a, uint8_t* ri
       for (int j = 0; j < PER; ++j) {
         if (first + j * STEP >= kKeysPerTile) break;
         const long long at = static_cast<long long>(rows[j]) * GROUPS + group;
-        const uint32_t codes = dst + (j * Form::PRODUCERS + id) * 32, words = dst + PER * Form::PRODUCERS * 32 + (j * Form::PRODUCERS + id) * 8;
+        const uint32_t codes = dst + (j * Form::PRODUCERS + id) * 16, words = dst + PER * Form::PRODUCERS * 32 + (j * Form::PRODUCERS + id) * 8;
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(codes), "l"(a.k_codes + at * 16) : "memory");
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(codes + 16), "l"(a.v_codes + at * 16) : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(codes + PER * Form::PRODUCERS * 16), "l"(a.v_codes + at * 16) : "memory");
         asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(words), "l"(a.k_words + (at & ~1LL)) : "memory");          // two groups' words
         asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(words + 4), "l"(a.v_words + (at & ~1LL)) : "memory");
       }
@@ -151,6 +157,11 @@ __device__ __forceinline__ void kv4_produce(const UmmaPromptArgs& a, uint8_t* ri
       *reinterpret_cast<uint4*>(dst + ((((group & 1) * 4 + c) ^ (row & 7)) << 4)) =
           make_uint4(kv4_low(w[c], s), kv4_high(w[c], s), kv4_low(next, s), kv4_high(next, s));
     }
+  };
+  const auto filled = [&](uint64_t* bar) {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if ((id & 31) == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
   };
   find(0);
 #pragma unroll 1
@@ -169,24 +180,31 @@ __device__ __forceinline__ void kv4_produce(const UmmaPromptArgs& a, uint8_t* ri
     for (int j = 0; j < PER; ++j) {
       const int key = (kt_first + i) * kKeysPerTile + first + j * STEP;
       if (first + j * STEP >= kKeysPerTile) break;
-      kc[j] = *reinterpret_cast<const uint4*>(src + (j * Form::PRODUCERS + id) * 32);
-      vc[j] = *reinterpret_cast<const uint4*>(src + (j * Form::PRODUCERS + id) * 32 + 16);
+      kc[j] = *reinterpret_cast<const uint4*>(src + (j * Form::PRODUCERS + id) * 16);
+      vc[j] = *reinterpret_cast<const uint4*>(src + ((PER + j) * Form::PRODUCERS + id) * 16);
       words[j] = *reinterpret_cast<const uint2*>(src + PER * Form::PRODUCERS * 32 + (j * Form::PRODUCERS + id) * 8);
       if (key < lo || key > hi) words[j] = make_uint2(0u, 0u);       // what no row sees: zeros
     }
     copy(i + Form::AHEAD);          // (this thread's own place, whose words it holds)
     find(i + Form::AHEAD + 1);
-    if (!__all_sync(0xffffffffu, mbar_wait(kv_empty + st, ((i / STAGES) & 1) ^ 1, abort_flag, a.status, 11) ? 1 : 0)) break;
     uint8_t* k_plane = ring + st * 2 * PLANE_BYTES;
+    if (!__all_sync(0xffffffffu, mbar_wait(kv_empty + st, ((i / STAGES) & 1) ^ 1, abort_flag, a.status, 11) ? 1 : 0)) break;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
       if (first + j * STEP >= kKeysPerTile) break;
       put(k_plane, first + j * STEP, kc[j], words[j].x);
-      put(k_plane + PLANE_BYTES, first + j * STEP, vc[j], words[j].y);
+      if (Form::RINGS == 1) put(k_plane + PLANE_BYTES, first + j * STEP, vc[j], words[j].y);
     }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    __syncwarp();
-    if ((id & 31) == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(kv_full + st)) : "memory");
+    if constexpr (Form::RINGS == 2) {
+      filled(kv_full + st);
+      if (!__all_sync(0xffffffffu, mbar_wait(kv_empty + STAGES + st, ((i / STAGES) & 1) ^ 1, abort_flag, a.status, 11) ? 1 : 0)) break;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        if (first + j * STEP >= kKeysPerTile) break;
+        put(k_plane + PLANE_BYTES, first + j * STEP, vc[j], words[j].y);
+      }
+    }
+    filled(kv_full + (Form::RINGS - 1) * STAGES + st);
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
@@ -195,7 +213,7 @@ template <typename Form>
 __global__ void __launch_bounds__(Form::THREADS, 1)
 attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, UmmaPromptArgs a) {
   pdl_sync();
-  constexpr int DH = Form::DH, STAGES = Form::STAGES, RT = Form::RT, TERMS = Form::TERMS;
+  constexpr int DH = Form::DH, STAGES = Form::STAGES, RINGS = Form::RINGS, RT = Form::RT, TERMS = Form::TERMS;
   constexpr bool KV4 = Form::KV4, F32 = Form::F32;
   constexpr int HALVES = DH / 64, P_BYTES = Form::P_BYTES, STAGE_BYTES = Form::STAGE_BYTES;
   constexpr int PLANE_BYTES = STAGE_BYTES / 2;    // 64 keys
@@ -212,8 +230,8 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
   uint8_t* ring = p_smem + Form::P_ALL;
   uint8_t* raw = ring + STAGES * STAGE_BYTES;      // KV4: codes and words on their way
   uint64_t* kv_full = reinterpret_cast<uint64_t*>(raw + (KV4 ? Form::AHEAD * Form::RAW : 0));
-  uint64_t* kv_empty = kv_full + STAGES;
-  uint64_t* s_full = kv_empty + STAGES;   // [2]
+  uint64_t* kv_empty = kv_full + RINGS * STAGES;
+  uint64_t* s_full = kv_empty + RINGS * STAGES;   // [2]
   uint64_t* s_empty = s_full + 2;
   uint64_t* p_full = s_empty + 2;         // [row tile][buffer]
   uint64_t* p_empty = p_full + 4;
@@ -256,7 +274,7 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
   const int n_tiles = kt_last - kt_first + 1;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < STAGES; ++s) {
+    for (int s = 0; s < RINGS * STAGES; ++s) {
       mbar_init(kv_full + s, KV4 ? Form::PRODUCERS / 32 : 1);
       mbar_init(kv_empty + s, 1);
     }
@@ -406,9 +424,9 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
       // i + 1, once it has taken the scores of tile i, which happens right behind that. The row tiles have waits of their own, so one's products
       // run while the other's softmax does: 8,192 tokens of 32 heads over 8 of 128 545 us, 649 with one wait for both row tiles' scores and one for
       // their weights. A wait costs this one thread a couple of hundred cycles even when the barrier has long flipped, so a row tile's are
-      // one (two: 606 us); but with KV4 and heads of 128, whose stages are three and filled by warps, P V and the stage's release come first
-      // (694 us against 815).
-      constexpr bool TOGETHER = !KV4 || (DH == 64 && RT == 2);
+      // one (two: 606 us); but where a few stages are filled by warps, P V and the stage's release come first (KV4, 4 portions of 512 at 2,048
+      // keys: heads of 128 98 us against 107, of 256 210 against 271; not of 192, 163 against 159).
+      constexpr bool TOGETHER = !KV4 || (DH == 64 && RT == 2) || DH == 192;
       const BarrierPhase none{nullptr, 0u, false};
       const auto wait = [&](const BarrierPhase& w0, const BarrierPhase& w1, const BarrierPhase& w2) {
         if (!w0.on && !w1.on && !w2.on) return;
@@ -422,17 +440,24 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
           const BarrierPhase keys{kv_full + (i + 1) % STAGES, static_cast<uint32_t>(((i + 1) / STAGES) & 1), q == 0 && i + 1 < n_tiles};
           const BarrierPhase taken{s_empty + q, static_cast<uint32_t>((n_qk[q] & 1) ^ 1), next};
           const BarrierPhase weights{p_full + 2 * q + (n_pv[q] & 1), static_cast<uint32_t>((n_pv[q] >> 1) & 1), last_one};
+          const BarrierPhase values{kv_full + STAGES + (i + STAGES - 1) % STAGES, static_cast<uint32_t>(((i - 1) / STAGES) & 1), RINGS == 2 && q == 0 && i >= 1};
           if (TOGETHER) wait(keys, taken, weights);
-          else wait(weights, none, none);
+          else wait(weights, values, none);
+          if (!ok) break;
+          if (RINGS == 2 && TOGETHER) wait(values, none, none);
           if (!ok) break;
           if (last_one) pv(q, i - 1);
-          if (q == RT - 1 && i >= 1) {        // all row tiles are done with key tile i - 1
-            if (elect_one()) umma_commit(kv_empty + (i - 1) % STAGES);
+          if (q == RT - 1 && i >= 1) {        // all row tiles are done with the values of key tile i - 1 (and with its keys)
+            if (elect_one()) umma_commit(kv_empty + (RINGS - 1) * STAGES + (i - 1) % STAGES);
             __syncwarp();
           }
           if (!TOGETHER) wait(keys, taken, none);
           if (!ok) break;
           if (next) qk(q, i + 1);
+          if (RINGS == 2 && q == RT - 1 && i + 1 < n_tiles) {      // with the keys of i + 1
+            if (elect_one()) umma_commit(kv_empty + (i + 1) % STAGES);
+            __syncwarp();
+          }
         }
       }
     }
@@ -720,8 +745,8 @@ static void cut_prompt_umma(UmmaPromptArgs& a, int max_queries, int n_seqs, int 
   int sms = 148;
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, 0);
   // ...; with many keys they share out the keys instead: what bounds either is the keys and values that L2 feeds the SMs, and tiles of
-  // 256 rows read them half as often. 128 rows a CTA against shares, us (with one wait for both row tiles, up to a tenth slower than now): two shares, 512 tokens of 32 heads over 8, heads of 128: 2,100
-  // keys 45 / 43, 3,000 57 / 51, 8,192 131 / 100, 16,384 246 / 175 (at 1,024 24 / 29: the merge costs about 8 us); heads of 64 37 / 37,
+  // 256 rows read them half as often. 128 rows a CTA against shares, us (with one wait for both row tiles, up to
+  // a tenth slower than now): two shares, 512 tokens of 32 heads over 8, heads of 128: 2,100 keys 45 / 43, 3,000 57 / 51, 8,192 131 / 100, 16,384 246 / 175 (at 1,024 24 / 29: the merge costs about 8 us); heads of 64 37 / 37,
   // 47 / 45, 111 / 92, 207 / 164. Four shares, 128 tokens: heads of 128 2,100 keys 43 / 37, 3,000 55 / 41, 8,192 126 / 65; 16 heads of 64 over
   // 4 35 / 31, 45 / 35, 104 / 57; 8 over 8 of 128 41 / 29, 53 / 31, 124 / 49.
   const long long ctas = static_cast<long long>(a.kv_heads) * ceil_div(max_rows, 256) * n_seqs;
