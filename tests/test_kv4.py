@@ -142,3 +142,11 @@ def test_designs_whose_mixers_know_no_4_bits_are_refused():
     cfg = plain_misudra.make_config([plain_misudra.latent_layer(mlp=plain_misudra.dense())])
     with pytest.raises(UnsupportedError, match="4 bits"):
         make_cache(Model(misudra_spec(parse_misudra_config(cfg)), torch.float32), num_pages=4, device="cpu", kv_bits=4)
+
+
+def test_queries_and_keys_in_place_refuse():
+    x, w, pos = torch.zeros(3, 256), torch.ones(64), torch.zeros(3, dtype=torch.int32)
+    for bad, why in (((x[:, :100], w, w, pos), "narrow"), ((x, w[:32], w, pos), "weights"), ((x, w, w.double(), pos), "weights"), ((x, w, w, pos[:2]), "positions"),
+                     ((x, w, w, pos.long()), "positions"), ((x, w, w, pos), "CUDA")):
+        refused(ops.qk_norm_rope, *bad[:3], 1e-6, 1e-6, None, bad[3], 2, 1, 64, match=why)
+    refused(ops.qk_norm_rope, x, w, w, 1e-6, 1e-6, w.double(), pos, 2, 1, 64, match="inv_freq")

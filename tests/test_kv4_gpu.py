@@ -401,6 +401,43 @@ def test_a_sequence_that_is_listed_twice():
     b.check(b.decode(seqs=[0, 1, 0]))
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("T,heads,kv_heads,head_dim,rot", [(1, 4, 2, 64, 64), (7, 8, 8, 128, 128), (300, 6, 2, 128, 128), (2050, 2, 1, 64, 64), (5, 3, 1, 48, 32), (260, 4, 2, 256, 0)])
+def test_queries_and_keys_prepared_in_place(dtype, T, heads, kv_heads, head_dim, rot):
+    """One launch over both does, bit for bit, what one over the queries and one over the keys do; values stay."""
+    rng = np.random.default_rng(T + head_dim)
+    width = (heads + 2 * kv_heads) * head_dim
+    x = cuda(rng.standard_normal((T, width)), DT[dtype])
+    qw, kw = (cuda(rng.random(head_dim) + 0.5, torch.float32) for _ in range(2))
+    table = cuda(10000.0 ** (-np.arange(0, rot, 2) / rot), torch.float32) if rot else None
+    pos = cuda(rng.integers(0, 40000, T))
+    want = x.clone()
+    q, k = want[:, :heads * head_dim], want[:, heads * head_dim:(heads + kv_heads) * head_dim]
+    ops.qk_norm_rope_append(q, qw, None, 1e-6, 0.0, table, pos, None, None, None, heads, kv_heads, head_dim, write_kv=False)
+    ops.qk_norm_rope_append(k, kw, None, 1e-5, 0.0, table, pos, None, None, None, kv_heads, kv_heads, head_dim, write_kv=False)
+    ops.qk_norm_rope(x, qw, kw, 1e-6, 1e-5, table, pos, heads, kv_heads, head_dim)
+    assert torch.equal(x, want)
+
+
+@pytest.mark.parametrize("T,heads,kv_heads,head_dim", [(1, 4, 2, 64), (9, 6, 2, 128), (3, 3, 1, 48)])
+def test_queries_and_keys_out_of_partial_sums(T, heads, kv_heads, head_dim):
+    """What goes back in place is what `qk_norm_rope_append` puts into a bfloat16 cache."""
+    rng = np.random.default_rng(T)
+    width = (heads + 2 * kv_heads) * head_dim
+    sums = ops.SplitSum(cuda(rng.standard_normal((3, T, width)), torch.float32).reshape(-1), 3, T, width)
+    qw, kw = (cuda(rng.random(head_dim) + 0.5, torch.float32) for _ in range(2))
+    table = cuda(10000.0 ** (-np.arange(0, head_dim, 2) / head_dim), torch.float32)
+    pos, slots = cuda(rng.integers(0, 40000, T)), cuda(np.arange(T))
+    got, want = (torch.zeros(T, width, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    planes = [torch.zeros(1, kv_heads, 16, head_dim, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    ops.qk_norm_rope_append(want, qw, kw, 1e-6, 1e-5, table, pos, slots, *planes, heads, kv_heads, head_dim, partial=sums)
+    ops.qk_norm_rope(got, qw, kw, 1e-6, 1e-5, table, pos, heads, kv_heads, head_dim, partial=sums)
+    for i, plane in enumerate(planes):
+        at = (heads + i * kv_heads) * head_dim
+        want[:, at:at + kv_heads * head_dim] = plane[0, :, :T].transpose(0, 1).reshape(T, -1)
+    assert torch.equal(got, want) and bool((got != 0).any(0).all())
+
+
 # ---- step tables
 
 def device_tables(requests, columns, pages):

@@ -378,20 +378,20 @@ __global__ void qk_norm_rope_append_kernel(T* __restrict__ qkv, long long row_st
   const bool is_q = head < q_heads;
   const bool is_k = !is_q && head < q_heads + kv_heads;
   T* dst = src;
-  if (!is_q) {
+  if (!is_q && k_cache != nullptr) {      // (no planes: keys and values go back in place)
     const int slot = slots[t];
     if (slot < 0) return;
     const int h = is_k ? head - q_heads : head - q_heads - kv_heads;
     const long long page = slot / page_size, off = slot % page_size;
     dst = (is_k ? k_cache : v_cache) + ((page * kv_heads + h) * page_size + off) * head_dim;
-    if (!is_k) {  // values are stored as they are
-      if (psrc) {
-        for (int i = lane; i < head_dim; i += 32) st(dst + i, value(i));
-      } else {
-        for (int i = lane; i < head_dim; i += 32) dst[i] = src[i];
-      }
-      return;
+  }
+  if (!is_q && !is_k) {  // values are stored as they are
+    if (psrc) {
+      for (int i = lane; i < head_dim; i += 32) st(dst + i, value(i));
+    } else {
+      for (int i = lane; i < head_dim; i += 32) dst[i] = src[i];
     }
+    return;
   }
 
   const float* w = is_q ? qw : kw;
@@ -446,7 +446,7 @@ __global__ void __launch_bounds__(256) qk_norm_rope_append_vec_kernel(T* __restr
   const bool is_q = head < q_heads;
   const bool is_k = !is_q && head < q_heads + kv_heads;
   T* dst = src;
-  if (!is_q) {
+  if (!is_q && k_cache != nullptr) {      // (no planes: keys and values go back in place)
     const int slot = slots[t];
     if (slot < 0) return;
     const int h = is_k ? head - q_heads : head - q_heads - kv_heads;
@@ -537,7 +537,7 @@ __global__ void __launch_bounds__(256, 4) qk_norm_rope_append_rows_kernel(T* __r
       const T* src = row + static_cast<long long>(head) * DH;
       T* dst = nullptr;
       if (head < heads_per_token) {
-        if (is_q) {
+        if (is_q || k_cache == nullptr) {
           dst = const_cast<T*>(src);
         } else if (slot >= 0) {
           const int h = is_v ? head - q_heads - kv_heads : head - q_heads;
@@ -677,7 +677,7 @@ int launch_qk_norm_rope_append(void* qkv, long long stride, const float* part, l
                                const float* inv_freq, int rot, const int* pos, const int* slots, void* kc, void* vc,
                                int tokens, int q_heads, int kv_heads, int head_dim, int page_size, int write_kv,
                                cudaStream_t s) {
-  const int heads_per_token = write_kv ? q_heads + 2 * kv_heads : q_heads;
+  const int heads_per_token = q_heads + (write_kv == 0 ? 0 : write_kv == 2 && part == nullptr ? kv_heads : 2 * kv_heads);
   const long long total = static_cast<long long>(tokens) * heads_per_token;
   if (total == 0) return kOk;
   const int warps = 8;
@@ -814,6 +814,7 @@ TIE_API int tie_kv_append(int dtype, const void* k, const void* v, long long k_s
                                                head_dim, page_size, s));
 }
 
+// write_kv 0: queries only; 1: keys and values into the planes; 2 (no planes): keys back in place, and values where they come from partial sums.
 TIE_API int tie_qk_norm_rope_append(int dtype, void* qkv, long long stride, const float* part, long long part_stride,
                                     int splits, long long part_ld, const float* qw, const float* kw,
                                     float q_eps, float k_eps, const float* inv_freq, int rot, const int* pos,

@@ -234,6 +234,25 @@ def qk_norm_rope_append(qkv: torch.Tensor, q_weight, k_weight, q_eps: float, k_e
          1 if write_kv else 0, _stream())
 
 
+def qk_norm_rope(qkv: torch.Tensor, q_weight, k_weight, q_eps: float, k_eps: float, inv_freq, positions: torch.Tensor, q_heads: int, kv_heads: int,
+                 head_dim: int, partial: SplitSum | None = None) -> None:
+    """What `qk_norm_rope_append` does to q and k, both back in place, in one launch: qkv [T, >= (q_heads + kv_heads) * head_dim], for caches that
+    take their keys from there (`kv4_append`). With `partial` q, k and v are read from the split product's partial sums and all
+    three written to qkv [T, >= (q_heads + 2 kv_heads) * head_dim]."""
+    T, width = qkv.shape[0], (q_heads + (1 if partial is None else 2) * kv_heads) * head_dim
+    _need(qkv.dim() == 2 and qkv.stride(1) == 1 and qkv.shape[1] >= width, "qk_norm_rope: qkv too narrow")
+    _need(positions.dtype == torch.int32 and positions.numel() == T, "qk_norm_rope: positions must be int32 [T]")
+    _need(all(w is None or (w.dtype == torch.float32 and w.numel() == head_dim) for w in (q_weight, k_weight)),
+          "qk_norm_rope: norm weights must be float32 [head_dim]")
+    _need(inv_freq is None or inv_freq.dtype == torch.float32, "qk_norm_rope: inv_freq must be float32")
+    _need(partial is None or (partial.M == T and partial.N == width), "qk_norm_rope: partial sums do not match the rows")
+    _dev(qkv, q_weight, k_weight, inv_freq, positions)
+    call("tie_qk_norm_rope_append", dtype_code(qkv), qkv.data_ptr(), qkv.stride(0), partial.partial.data_ptr() if partial else 0,
+         partial.stride if partial else 0, partial.splits if partial else 0, partial.N if partial else 0, _ptr(q_weight), _ptr(k_weight), float(q_eps),
+         float(k_eps), _ptr(inv_freq), 0 if inv_freq is None else 2 * inv_freq.numel(), positions.data_ptr(), 0, 0, 0, T, q_heads, kv_heads, head_dim, 1, 2,
+         _stream())
+
+
 def gemm_simt(a: torch.Tensor, w: torch.Tensor, out: torch.Tensor) -> None:
     """out[M, N] = a[M, K] . w[N, K]^T on the CUDA cores with float accumulation (any sizes)."""
     _dev(a, w, out)

@@ -15,6 +15,7 @@ to stay below 2^57 in magnitude; what they hold below 2^-62 it may lose.
 """
 from __future__ import annotations
 
+import os
 from typing import NamedTuple
 
 import torch
@@ -94,6 +95,7 @@ def _fail(msg: str):
 # groups) 18 and 10, 128 at 1,024 (256 groups) 29 and 20, at 2,048 35 and 44, 192 at 1,024 (384 groups) 29 and 33, 512 at 512 20 and 38; 4
 # of 512 at 2,048 98 and 396. float32: 64 at 300 20 and 11, 192 at 1,024 34 and 44, 4 of 512 at 2,048 195 and 646.
 UMMA_MIN_ROWS, UMMA_GROUPS, UMMA_FEW_GROUPS = 48, 384, 128
+_NO_UMMA_ATTENTION = os.environ.get("TIE_NO_UMMA_ATTENTION") == "1"
 _FLOATS = {torch.float32: 0, torch.bfloat16: 1}
 _I32 = torch.int32
 
@@ -264,7 +266,7 @@ def attention_kv4_decode(q, cache: Kv4Cache, out, query_start, context_lens, blo
 
 def _on_tcgen05(dtype, sizes, T, group, n_seqs, max_queries, keys):
     rows, head_dim = max_queries * group, sizes[1]
-    if rows < UMMA_MIN_ROWS or head_dim > (256 if dtype else 128) or head_dim % 8 or n_seqs > 16383 or rows > 65535 * 128:
+    if _NO_UMMA_ATTENTION or rows < UMMA_MIN_ROWS or head_dim > (256 if dtype else 128) or head_dim % 8 or n_seqs > 16383 or rows > 65535 * 128:
         return False
     groups = sizes[0] * min(n_seqs * ((rows + 15) // 16), T * group // 16 + n_seqs)
     return groups >= UMMA_GROUPS or (groups >= UMMA_FEW_GROUPS and groups * keys >= UMMA_GROUPS * 1024)

@@ -108,19 +108,19 @@ class GQAttention(Mixer):
                 self._capacity = (ops.partial_capacity(ctx.ws.max_rows, self.gemm_qkv.N, self.gemm_qkv.K, split_many=False),
                                   ops.partial_capacity(ctx.ws.max_rows, self.gemm_o.N, self.gemm_o.K))
             product = self.gemm_qkv if cache.writes else self.gemm_q
-            if cache.kv4 is not None:
-                product(h, qkv)
-                q, k = qkv[:, :self.q_dim], qkv[:, self.q_dim:self.q_dim + self.kv_dim]
-                ops.qk_norm_rope_append(q, qw, None, q_eps, 0.0, table, ctx.positions, None, None, None, Hq, Hkv, Dh, write_kv=False)
-                if cache.writes:
-                    ops.qk_norm_rope_append(k, kw, None, k_eps, 0.0, table, ctx.positions, None, None, None, Hkv, Hkv, Dh, write_kv=False)
-                    ops.kv4_append(k, qkv[:, self.q_dim + self.kv_dim:], g.slots, cache.kv4)
-                attn = ctx.ws.rows("attn.out", T, self.q_dim, self.dtype)
-                self.attend(q, attn, ctx, g, cache)
-                return self.output(attn, ctx)
             got = product(
                 h, qkv, lambda n: ctx.ws.flat("attn.qkv.partial", n, torch.float32, self._capacity[0]))
             partial = got if isinstance(got, ops.SplitSum) else None
+            if cache.kv4 is not None:
+                q = qkv[:, :self.q_dim]
+                if cache.writes:
+                    ops.qk_norm_rope(qkv, qw, kw, q_eps, k_eps, table, ctx.positions, Hq, Hkv, Dh, partial=partial)
+                    ops.kv4_append(qkv[:, self.q_dim:self.q_dim + self.kv_dim], qkv[:, self.q_dim + self.kv_dim:], g.slots, cache.kv4)
+                else:
+                    ops.qk_norm_rope_append(q, qw, None, q_eps, 0.0, table, ctx.positions, None, None, None, Hq, Hkv, Dh, write_kv=False, partial=partial)
+                attn = ctx.ws.rows("attn.out", T, self.q_dim, self.dtype)
+                self.attend(q, attn, ctx, g, cache)
+                return self.output(attn, ctx)
             if ctx.multi_rows == 0 and ops.attention_decode_prep_takes(qkv, Hq, Hkv, Dh, cache.k.shape[2], table):
                 # every sequence brings one token: the attention kernel prepares the heads itself
                 attn = ctx.ws.rows("attn.out", T, self.q_dim, self.dtype)
