@@ -11,11 +11,11 @@
 // One CTA owns 256 rows (rows = queries x the query heads of one kv head) as two tiles of 128, so
 // that the tensor cores work on one tile while the other tile's softmax runs, and both share every
 // key/value tile of 64 keys. The MMAs' operand reads are what shared memory has to feed, so Q, which
-// every key tile needs again, sits in tensor memory (the A operand of Q K^T comes from there) and only
-// K, V and P are read from shared memory. Ten warps:
+// every key tile needs again, sits in tensor memory (the A operand of Q K^T comes from there), P too where
+// it has room, and only K, V and else P are read from shared memory. Ten warps:
 //   0-3, 4-7  softmax of tile 0 and 1: thread = one row. Puts its Q row into tensor memory once. Per key
 //             tile it reads its 64 scores out of tensor memory, masks, exponentiates in float, writes P as
-//             bfloat16 into one of two shared-memory buffers (the layout the MMA reads) and keeps the row
+//             bfloat16 into one of two buffers (in shared memory in the layout the MMA reads) and keeps the row
 //             sum. The accumulator O stays in tensor memory; it is rescaled only when a row's maximum has
 //             grown by more than 2^8 since the value it was last scaled for (any reference point gives
 //             the same O / sum, as long as nothing overflows).
@@ -33,8 +33,8 @@
 // Warps take the place of the TMA producer: they read codes and words some tiles ahead, take them apart and write the
 // tile as TMA would have. Heads above 128 leave tensor memory for one row tile a CTA; so do float queries, which
 // stand there as three bfloat16 terms (24 bits), as the weights do in shared memory. 4 portions of 512 queries at 2,048 keys, 32 heads over 8,
-// us against the kernel whose warps take 16 rows each: heads of 128 98 and 396 (float 195 and 646), of 64 87 and 267 (162 and 407), of 192
-// 159 and 589, of 256 210 and 790. Eight dimensions lie in a tile in the order 0 4 1 5 2 6 3 7, in which a word of codes comes apart; Q is put into tensor
+// us against the kernel whose warps take 16 rows each: heads of 128 98 and 396 (float 195 and 646), of 64 79 and 267 (149 and 407), of 192
+// 148 and 589, of 256 192 and 790. Eight dimensions lie in a tile in the order 0 4 1 5 2 6 3 7, in which a word of codes comes apart; Q is put into tensor
 // memory in the same order and the outputs are taken out of it again. Keys and values are exact in bfloat16, times 2^-64 (kv4.cuh).
 #include "attention_mma.cuh"
 #include "kv4.cuh"
@@ -94,11 +94,15 @@ struct UmmaForm {
   static constexpr int RAW = ROUNDS * PRODUCERS * 40;             // bytes of a tile on its way: a thread's two times 16 bytes of codes and two words
   // Pairs of barriers a stage: 1 for keys and values together; 2 with one for the keys, which are filled again while the values are still read. That
   // pays where the producers are what the others wait for (4 portions of 512 queries at 2,048 keys, 32 heads over 8 of 256: 210 us instead of
-  // 235, of 64: 87 instead of 91) and else costs waits (of 128: 109 instead of 98; of 192: 174 instead of 159).
+  // 235, of 64: 87 instead of 91, with P in shared memory) and else costs waits (of 128: 109 instead of 98; of 192: 174 instead of 159).
   static constexpr int RINGS = KV4_ && !F32_ && (DH <= 64 || DH == 256) ? 2 : 1;
   static constexpr int P_BYTES = 128 * 128;                       // 128 rows x 64 keys
   static constexpr int STAGE_BYTES = 2 * (DH / 64) * 64 * 128;    // keys and values of a tile
-  static constexpr int P_ALL = RT * 2 * TERMS * P_BYTES;          // [row tile][buffer][term]
+  // Where its 512 columns hold scores, Q, accumulators and two tiles' weights P (32 columns a term), P stands in tensor memory too: nothing to store
+  // in shared memory and to read there again (KV4, 4 portions of 512 at 2,048 keys: heads of 64 79 us instead of 87, of 192 148 instead of 159,
+  // of 256 192 instead of 211, float of 64 149 instead of 163; bfloat16 pages, 16 heads of 64 over 4 at 8,192 keys 138 instead of 170).
+  static constexpr bool P_TMEM = RT * (64 + TERMS * DH / 2 + DH + 64 * TERMS) <= 512;
+  static constexpr int P_ALL = P_TMEM ? 0 : RT * 2 * TERMS * P_BYTES;         // [row tile][buffer][term]
   static constexpr int SMEM = P_ALL + STAGES * STAGE_BYTES + (KV4 ? AHEAD * RAW : 0) + (2 * RINGS * STAGES + 12) * 8 + 16 + 1024;
   static_assert(SMEM <= 227 * 1024, "shared memory of one CTA");
   static_assert(SMEM >= RT * 128 * (DH + 4) * 4 + (2 * RINGS * STAGES + 12) * 8 + 16 + 1024, "the sums of a CTA's rows");
@@ -113,7 +117,7 @@ __device__ __forceinline__ void kv4_produce(const UmmaPromptArgs& a, uint8_t* ri
   constexpr int GROUPS = Form::DH / 32, PER = Form::ROUNDS, RAW = Form::RAW, STAGES = Form::STAGES, PLANE_BYTES = Form::STAGE_BYTES / 2;
   static_assert(Form::PRODUCERS % (4 * GROUPS) == 0, "a thread's keys have one group");
   // Eight threads have four keys' 64 dimensions: what they store at a time lies in eight different places of a row of 128 bytes. (With a key's groups
-  // side by side it lies in two to four: heads of 256 330 us instead of 235, of 192 203 instead of 159, of 128 105 instead of 98, as above.)
+  // side by side it lies in two to four: with P in shared memory heads of 256 330 us instead of 235, of 192 203 instead of 159, of 128 105 instead of 98.)
   const int group = (id >> 3) % (GROUPS / 2) * 2 + (id & 1), first = (id >> 3) / (GROUPS / 2) * 4 + ((id >> 1) & 3);
   constexpr int STEP = Form::PRODUCERS / GROUPS;                  // its keys: first + j * STEP of a tile, below its 64
   const int* table = a.block_tables + static_cast<long long>(seq) * a.max_blocks;
@@ -214,12 +218,13 @@ __global__ void __launch_bounds__(Form::THREADS, 1)
 attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, UmmaPromptArgs a) {
   pdl_sync();
   constexpr int DH = Form::DH, STAGES = Form::STAGES, RINGS = Form::RINGS, RT = Form::RT, TERMS = Form::TERMS;
-  constexpr bool KV4 = Form::KV4, F32 = Form::F32;
+  constexpr bool KV4 = Form::KV4, F32 = Form::F32, P_TMEM = Form::P_TMEM;
   constexpr int HALVES = DH / 64, P_BYTES = Form::P_BYTES, STAGE_BYTES = Form::STAGE_BYTES;
   constexpr int PLANE_BYTES = STAGE_BYTES / 2;    // 64 keys
   // columns: the row tiles' scores, their Q (two elements a column, a term behind the other), their accumulators; of one row tile the
   // accumulator first
   constexpr int S_COL = RT == 1 ? DH : 0, Q_COL = S_COL + 64 * RT, O_COL = RT == 1 ? 0 : Q_COL + RT * TERMS * DH / 2;
+  constexpr int P_COL = RT * (64 + TERMS * DH / 2 + DH);      // P_TMEM: [row tile][buffer][term]
   constexpr uint32_t TMEM_COLS = 512;
   static_assert(64 * RT + RT * TERMS * DH / 2 + RT * DH <= 512, "tensor memory");
   constexpr float kRescaleStep = 8.0f;
@@ -411,8 +416,10 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
           for (int term = TERMS - 1; term >= 0; --term) {
 #pragma unroll
             for (int kk = 0; kk < kKeysPerTile / 16; ++kk) {
-              umma_bf16(tmem_base + O_COL + q * DH, desc_from_words(p_lo + ((term * P_BYTES + kk * 32) >> 4), kDescHiSw128),
-                        desc_from_words(v_lo + ((kk * 16 * 128) >> 4), kDescHiSw128), idesc_pv, kk > 0 || term < TERMS - 1 ? 1u : keep);
+              const uint64_t v_desc = desc_from_words(v_lo + ((kk * 16 * 128) >> 4), kDescHiSw128);
+              const uint32_t add = kk > 0 || term < TERMS - 1 ? 1u : keep;
+              if constexpr (P_TMEM) umma_bf16_a_tmem(tmem_base + O_COL + q * DH, tmem_base + P_COL + (pb * TERMS + term) * 32 + kk * 8, v_desc, idesc_pv, add);
+              else umma_bf16(tmem_base + O_COL + q * DH, desc_from_words(p_lo + ((term * P_BYTES + kk * 32) >> 4), kDescHiSw128), v_desc, idesc_pv, add);
             }
           }
           umma_commit(p_empty + pb);
@@ -547,9 +554,11 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
       // this buffer held P of the tile before the last one: its P V has to have retired
       const int pb = 2 * q + (n & 1);
       uint8_t* p_row = p_rows + (n & 1) * TERMS * P_BYTES;
+      const uint32_t p_tmem = tmem_base + lane_base + P_COL + pb * TERMS * 32;
       if constexpr (F32) {
         ok = __all_sync(0xffffffffu, mbar_wait(p_empty + pb, ((n >> 1) & 1) ^ 1, abort_flag, a.status, 13) ? 1 : 0) != 0;
         if (!ok) break;
+        if constexpr (P_TMEM) asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
           uint32_t w[TERMS][4];
@@ -564,8 +573,10 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
             for (int term = 0; term < TERMS; ++term) w[term][e] = terms[term];
           }
 #pragma unroll
-          for (int term = 0; term < TERMS; ++term)
-            *reinterpret_cast<uint4*>(p_row + term * P_BYTES + ((c ^ (rr & 7)) << 4)) = make_uint4(w[term][0], w[term][1], w[term][2], w[term][3]);
+          for (int term = 0; term < TERMS; ++term) {
+            if constexpr (P_TMEM) tmem_st4(p_tmem + term * 32 + 4 * c, w[term]);
+            else *reinterpret_cast<uint4*>(p_row + term * P_BYTES + ((c ^ (rr & 7)) << 4)) = make_uint4(w[term][0], w[term][1], w[term][2], w[term][3]);
+          }
         }
       } else {
 #pragma unroll
@@ -580,12 +591,22 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
         }
         ok = __all_sync(0xffffffffu, mbar_wait(p_empty + pb, ((n >> 1) & 1) ^ 1, abort_flag, a.status, 13) ? 1 : 0) != 0;
         if (!ok) break;
+        if constexpr (P_TMEM) {
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          uint32_t w0[16], w1[16];
 #pragma unroll
-        for (int c = 0; c < 8; ++c)
-          *reinterpret_cast<uint4*>(p_row + ((c ^ (rr & 7)) << 4)) = make_uint4(sr[4 * c], sr[4 * c + 1], sr[4 * c + 2], sr[4 * c + 3]);
+          for (int e = 0; e < 16; ++e) w0[e] = sr[e], w1[e] = sr[16 + e];
+          tmem_st16(p_tmem, w0);
+          tmem_st16(p_tmem + 16, w1);
+        } else {
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            *reinterpret_cast<uint4*>(p_row + ((c ^ (rr & 7)) << 4)) = make_uint4(sr[4 * c], sr[4 * c + 1], sr[4 * c + 2], sr[4 * c + 3]);
+        }
       }
       l += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      if constexpr (P_TMEM) asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      else asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
       if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(p_full + pb)) : "memory");
