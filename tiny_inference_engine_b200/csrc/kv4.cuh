@@ -84,6 +84,31 @@ __device__ __forceinline__ void load8(const T* p, int dims, bool vec, float (&x)
   }
 }
 
+// Two floats that sm_100a works on as one.
+using Pair = unsigned long long;
+__device__ __forceinline__ Pair pair(float a, float b) {
+  Pair d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float low_of(Pair p) { return __uint_as_float(static_cast<uint32_t>(p)); }
+__device__ __forceinline__ float high_of(Pair p) { return __uint_as_float(static_cast<uint32_t>(p >> 32)); }
+__device__ __forceinline__ Pair fma_pair(Pair a, Pair b, Pair c) {
+  Pair d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ Pair mul_pair(Pair a, Pair b) {
+  Pair d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ Pair add_pair(Pair a, Pair b) {
+  Pair d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
 // The smallest number of three significant bits that is not below (hi - lo) / 15; the float division rounds first.
 __device__ __forceinline__ float kv4_step(float lo, float hi) {
   const float least = fmaxf(__fdiv_rn(hi - lo, 15.0f), kKv4LeastScale);

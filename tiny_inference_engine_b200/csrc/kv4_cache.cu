@@ -55,29 +55,6 @@ __device__ __forceinline__ float min_nan(float a, float b, float c) {
   return d;
 }
 
-// Two floats that sm_100a works on as one.
-using Pair = unsigned long long;
-__device__ __forceinline__ Pair pair(float a, float b) {
-  Pair d;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
-  return d;
-}
-__device__ __forceinline__ Pair fma_pair(Pair a, Pair b, Pair c) {
-  Pair d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ Pair mul_pair(Pair a, Pair b) {
-  Pair d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ Pair add_pair(Pair a, Pair b) {
-  Pair d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-
 // Eight values as codes. Four codes are the digits of one number, whose bits 2^23 shows; dimensions 0-3 and 4-7 side by side.
 // rint(x / s) >= rint(lo / s) = -z, and rint(x / s) + z is above 15 only where both x / s and -lo / s are halves that round up, and then
 // 16: `top` says so for the group.
