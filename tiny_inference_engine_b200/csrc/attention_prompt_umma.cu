@@ -33,8 +33,8 @@
 // Warps take the place of the TMA producer: they read codes and words some tiles ahead, take them apart and write the
 // tile as TMA would have. Heads above 128 leave tensor memory for one row tile a CTA; so do float queries, which
 // stand there as three bfloat16 terms (24 bits), as the weights do in shared memory. 4 portions of 512 queries at 2,048 keys, 32 heads over 8,
-// us against the kernel whose warps take 16 rows each: heads of 128 98 and 396 (float 195 and 646), of 64 79 and 267 (149 and 407), of 192
-// 148 and 589, of 256 192 and 790. Eight dimensions lie in a tile in the order 0 4 1 5 2 6 3 7, in which a word of codes comes apart; Q is put into tensor
+// us against the kernel whose warps take 16 rows each: heads of 128 97 and 396 (float 195 and 646), of 64 77 and 267 (149 and 407), of 192
+// 148 and 589, of 256 189 and 790. Eight dimensions lie in a tile in the order 0 4 1 5 2 6 3 7, in which a word of codes comes apart; Q is put into tensor
 // memory in the same order and the outputs are taken out of it again. Keys and values are exact in bfloat16, times 2^-64 (kv4.cuh).
 #include "attention_mma.cuh"
 #include "kv4.cuh"
