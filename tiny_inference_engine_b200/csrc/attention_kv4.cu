@@ -1,5 +1,5 @@
-// Attention over a cache in 4 bits (the format: kv4.cuh) for few rows at a time: sequences that bring one token, short portions, the 32-bit
-// path, and every head size up to 256. Long bfloat16 portions of heads up to 128 run in attention_prompt_umma.cu.
+// Attention over a cache in 4 bits (the format: kv4.cuh) for few rows at a time: sequences that bring one token, short portions, rows and heads of
+// any alignment and size up to 256. Long portions run in attention_prompt_umma.cu (bfloat16 heads up to 256, float up to 128).
 //
 // What it computes, for row (query j of sequence s, head h): pos = context - queries + j, keys lo..pos (lo > 0 only with a window),
 //     out = sum_k softmax_k(scale q . K_k) V_k,   K_k, V_k the bfloat16 values that the codes stand for;  no key: zeros.
@@ -613,7 +613,7 @@ TIE_API int tie_attention_kv4(int dtype, const void* q, long long q_stride, long
   if (splits > 128) splits = 128;             // (four a lane in the merge)
   if (splits < 1) splits = 1;
   int shift = 0;
-  while ((1 << shift) < page_size) ++shift;
+  while (shift < 30 && (1 << shift) < page_size) ++shift;
   if ((1 << shift) != page_size) shift = -1;
   const int size = f32 ? 4 : 2;
   const int q_aligned = reinterpret_cast<uintptr_t>(q) % 16 == 0 && q_stride * size % 16 == 0 && head_dim * size % 16 == 0;

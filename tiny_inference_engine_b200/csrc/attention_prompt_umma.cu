@@ -860,7 +860,7 @@ TIE_API int tie_attention_prompt_kv4(int dtype, const void* q, long long q_strid
   TIE_REQUIRE(all_rows <= 65535LL * 128, "attention_prompt_kv4: %d queries in one portion are too many", max_queries);
   TIE_REQUIRE(status_word() != nullptr, "attention_prompt_kv4: cannot allocate the status word");
   int shift = 0;
-  while ((1 << shift) < page_size) ++shift;
+  while (shift < 30 && (1 << shift) < page_size) ++shift;
   if ((1 << shift) != page_size) shift = -1;
   UmmaPromptArgs a{static_cast<const __nv_bfloat16*>(q), static_cast<__nv_bfloat16*>(out), query_start, context_lens, block_tables, status_word(), q_stride, max_blocks,
                    q_heads, kv_heads, page_size, shift, window, scale * 1.4426950408889634f * kKv4Unscale, 1, 256, static_cast<const uint8_t*>(k_codes),

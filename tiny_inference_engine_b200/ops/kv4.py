@@ -93,7 +93,7 @@ def _fail(msg: str):
 # slower (9 to 15 us a call against 5 to 10) and its tiles of 128 rows are too few for the GPU until then. bfloat16, 32 heads over 8 of 128, us with
 # it and without: 64 portions of 16 rows at 512 keys 69 and 26, 32 of 48 rows at 64 18 and 21, 16 of 64 rows 10 and 15; one of 64 queries at 300 keys (128
 # groups) 18 and 10, 128 at 1,024 (256 groups) 29 and 20, at 2,048 35 and 44, 192 at 1,024 (384 groups) 29 and 33, 512 at 512 20 and 38; 4
-# of 512 at 2,048 98 and 396. float32: 64 at 300 20 and 11, 192 at 1,024 34 and 44, 4 of 512 at 2,048 195 and 646.
+# of 512 at 2,048 97 and 396. float32: 64 at 300 20 and 11, 192 at 1,024 34 and 44, 4 of 512 at 2,048 195 and 646.
 UMMA_MIN_ROWS, UMMA_GROUPS, UMMA_FEW_GROUPS = 48, 384, 128
 _NO_UMMA_ATTENTION = os.environ.get("TIE_NO_UMMA_ATTENTION") == "1"
 _FLOATS = {torch.float32: 0, torch.bfloat16: 1}
