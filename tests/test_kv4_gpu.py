@@ -382,6 +382,35 @@ def test_other_streams_and_graphs():
     assert np.array_equal(want, b.answer())
 
 
+@pytest.mark.parametrize("dtype,head_dim,contexts", [("bfloat16", 64, [3000]), ("bfloat16", 128, [700, 300]), ("bfloat16", 256, [3000]), ("float32", 128, [2500])])
+def test_long_portions_on_other_streams_and_in_graphs(monkeypatch, dtype, head_dim, contexts):
+    """With the keys in one share and in several; queries and contexts that change between replays are the ones that count."""
+    monkeypatch.setattr(kv4, "UMMA_GROUPS", 0)
+    b = Batch(41, contexts, [130] * len(contexts), 4, 2, head_dim, 16, dtype, pad=8)
+    want = b.prompt()
+    b.check(want, one_term=True, truncated=True)
+    args = len(contexts), 130, b.heads, b.scale, max(contexts), b.work
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        b.out.fill_(0.0)
+        ops.attention_kv4_prompt(b.qt, b.cache, b.out, *b.args, *args)
+    side.synchronize()
+    assert np.array_equal(want, b.answer())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.attention_kv4_prompt(b.qt, b.cache, b.out, *b.args, *args)
+    b.args[1].sub_(140)         # fewer keys: every row sees other ones
+    graph.replay()
+    fewer = b.answer()
+    ops.attention_kv4_prompt(b.qt, b.cache, b.out, *b.args, *args)
+    assert np.array_equal(fewer, b.answer()) and not np.array_equal(fewer, want)
+    b.args[1].add_(140)
+    b.out.fill_(0.0)
+    graph.replay()
+    assert np.array_equal(want, b.answer())
+
+
 def test_calls_at_the_same_time_with_workspaces_of_their_own():
     batches = [Batch(20 + i, [4000, 300, 2500], [1] * 3, 8, 2, 128, 16, "bfloat16") for i in range(2)]
     want = [b.decode() for b in batches]
