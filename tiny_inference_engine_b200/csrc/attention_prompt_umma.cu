@@ -11,11 +11,11 @@
 // One CTA owns 256 rows (rows = queries x the query heads of one kv head) as two tiles of 128, so
 // that the tensor cores work on one tile while the other tile's softmax runs, and both share every
 // key/value tile of 64 keys. The MMAs' operand reads are what shared memory has to feed, so Q, which
-// every key tile needs again, sits in tensor memory (the A operand of Q K^T comes from there), P too where
-// it has room, and only K, V and else P are read from shared memory. Ten warps:
+// every key tile needs again, sits in tensor memory (the A operand of Q K^T comes from there; of heads of 128 one half), P too
+// where it has room, and only K, V and what has none are read from shared memory. Ten warps:
 //   0-3, 4-7  softmax of tile 0 and 1: thread = one row. Puts its Q row into tensor memory once. Per key
 //             tile it reads its 64 scores out of tensor memory, masks, exponentiates in float, writes P as
-//             bfloat16 into one of two buffers (in shared memory in the layout the MMA reads) and keeps the row
+//             bfloat16 into one of its buffers (in shared memory in the layout the MMA reads) and keeps the row
 //             sum. The accumulator O stays in tensor memory; it is rescaled only when a row's maximum has
 //             grown by more than 2^8 since the value it was last scaled for (any reference point gives
 //             the same O / sum, as long as nothing overflows).
@@ -33,7 +33,7 @@
 // Warps take the place of the TMA producer: they read codes and words some tiles ahead, take them apart and write the
 // tile as TMA would have. Heads above 128 leave tensor memory for one row tile a CTA; so do float queries, which
 // stand there as three bfloat16 terms (24 bits), as the weights do in shared memory. 4 portions of 512 queries at 2,048 keys, 32 heads over 8,
-// us against the kernel whose warps take 16 rows each: heads of 128 97 and 396 (float 195 and 646), of 64 77 and 267 (149 and 407), of 192
+// us against the kernel whose warps take 16 rows each: heads of 128 88 and 396 (float 195 and 646), of 64 77 and 267 (149 and 407), of 192
 // 148 and 589, of 256 189 and 790. Eight dimensions lie in a tile in the order 0 4 1 5 2 6 3 7, in which a word of codes comes apart; Q is put into tensor
 // memory in the same order and the outputs are taken out of it again. Keys and values are exact in bfloat16, times 2^-64 (kv4.cuh).
 #include "attention_mma.cuh"
@@ -100,9 +100,13 @@ struct UmmaForm {
   static constexpr int STAGE_BYTES = 2 * (DH / 64) * 64 * 128;    // keys and values of a tile
   // Where its 512 columns hold scores, Q, accumulators and two tiles' weights P (32 columns a term), P stands in tensor memory too: nothing to store
   // in shared memory and to read there again (KV4, 4 portions of 512 at 2,048 keys: heads of 64 79 us instead of 87, of 192 148 instead of 159,
-  // of 256 192 instead of 211, float of 64 149 instead of 163; bfloat16 pages, 16 heads of 64 over 4 at 8,192 keys 138 instead of 170).
-  static constexpr bool P_TMEM = RT * (64 + TERMS * DH / 2 + DH + 64 * TERMS) <= 512;
-  static constexpr int P_ALL = P_TMEM ? 0 : RT * 2 * TERMS * P_BYTES;         // [row tile][buffer][term]
+  // of 256 192 instead of 211, float of 64 149 instead of 163; bfloat16 pages, 16 heads of 64 over 4 at 8,192 keys 138 instead of 170). Two row tiles with heads of
+  // 128 make room for one tile's weights each by leaving the second half of Q in shared memory, which is written once (88 us instead of 97; bfloat16
+  // pages, 512 queries of 32 heads over 8 at 8,192 keys 85 instead of 98).
+  static constexpr bool Q_HALF = DH == 128 && RT == 2;
+  static constexpr int Q_COLS = TERMS * DH / 2 / (Q_HALF ? 2 : 1), P_BUFS = Q_HALF ? 1 : 2;
+  static constexpr bool P_TMEM = RT * (64 + Q_COLS + DH + 32 * P_BUFS * TERMS) <= 512;
+  static constexpr int P_ALL = Q_HALF ? RT * P_BYTES : P_TMEM ? 0 : RT * 2 * TERMS * P_BYTES;         // [row tile][buffer][term]
   static constexpr int SMEM = P_ALL + STAGES * STAGE_BYTES + (KV4 ? AHEAD * RAW : 0) + (2 * RINGS * STAGES + 12) * 8 + 16 + 1024;
   static_assert(SMEM <= 227 * 1024, "shared memory of one CTA");
   static_assert(SMEM >= RT * 128 * (DH + 4) * 4 + (2 * RINGS * STAGES + 12) * 8 + 16 + 1024, "the sums of a CTA's rows");
@@ -223,15 +227,16 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
   constexpr int PLANE_BYTES = STAGE_BYTES / 2;    // 64 keys
   // columns: the row tiles' scores, their Q (two elements a column, a term behind the other), their accumulators; of one row tile the
   // accumulator first
-  constexpr int S_COL = RT == 1 ? DH : 0, Q_COL = S_COL + 64 * RT, O_COL = RT == 1 ? 0 : Q_COL + RT * TERMS * DH / 2;
-  constexpr int P_COL = RT * (64 + TERMS * DH / 2 + DH);      // P_TMEM: [row tile][buffer][term]
+  constexpr int S_COL = RT == 1 ? DH : 0, Q_COL = S_COL + 64 * RT, O_COL = RT == 1 ? 0 : Q_COL + RT * Form::Q_COLS;
+  constexpr int P_COL = RT * (64 + Form::Q_COLS + DH), P_BUFS = Form::P_BUFS, Q_COLS = Form::Q_COLS;
+  constexpr bool Q_HALF = Form::Q_HALF;      // P_TMEM: [row tile][buffer][term]
   constexpr uint32_t TMEM_COLS = 512;
-  static_assert(64 * RT + RT * TERMS * DH / 2 + RT * DH <= 512, "tensor memory");
+  static_assert(64 * RT + RT * Form::Q_COLS + RT * DH <= 512, "tensor memory");
   constexpr float kRescaleStep = 8.0f;
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);      // (an offset, so that the compiler still sees shared memory)
-  uint8_t* p_smem = smem;                 // [row tile][buffer][term]
+  uint8_t* p_smem = smem;                 // [row tile][buffer][term]; Q_HALF: dimensions 64.. of Q, [row tile]
   uint8_t* ring = p_smem + Form::P_ALL;
   uint8_t* raw = ring + STAGES * STAGE_BYTES;      // KV4: codes and words on their way
   uint64_t* kv_full = reinterpret_cast<uint64_t*>(raw + (KV4 ? Form::AHEAD * Form::RAW : 0));
@@ -309,7 +314,7 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
     const int head_dim = KV4 ? a.head_dim : DH;
     const bool there = row < rows && (!KV4 || t0 + row / G < a.tokens);
     const long long at = there ? static_cast<long long>(t0 + row / G) * a.q_stride + static_cast<long long>(kvh * G + row % G) * head_dim : 0;
-    const uint32_t q_tmem = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16) + Q_COL + q * TERMS * (DH / 2);
+    const uint32_t q_tmem = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16) + Q_COL + q * Q_COLS;
 #pragma unroll
     for (int c0 = 0; c0 < DH / 2; c0 += 16) {
       uint32_t w[TERMS][16];
@@ -338,9 +343,18 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
         }
       }
 #pragma unroll
-      for (int term = 0; term < TERMS; ++term) tmem_st16(q_tmem + term * (DH / 2) + c0, w[term]);
+      for (int term = 0; term < TERMS; ++term) {
+        if (Q_HALF && c0 >= DH / 4) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            *reinterpret_cast<uint4*>(p_smem + q * P_BYTES + rr * 128 + (((c0 - DH / 4) / 4 + e) ^ (rr & 7)) * 16) = make_uint4(w[0][4 * e], w[0][4 * e + 1], w[0][4 * e + 2], w[0][4 * e + 3]);
+        } else {
+          tmem_st16(q_tmem + term * (DH / 2) + c0, w[term]);
+        }
+      }
     }
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+    if (Q_HALF) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
@@ -396,9 +410,10 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
           for (int term = TERMS - 1; term >= 0; --term) {
 #pragma unroll
             for (int ks = 0; ks < DH / 16; ++ks) {
-              umma_bf16_a_tmem(tmem_base + S_COL + q * kKeysPerTile, tmem_base + Q_COL + (q * TERMS + term) * (DH / 2) + ks * 8,
-                               desc_from_words(k_lo + (((ks >> 2) * (64 * 128) + (ks & 3) * 32) >> 4), kDescHiSw128), idesc_qk,
-                               ks > 0 || term < TERMS - 1 ? 1u : 0u);
+              const uint64_t k_desc = desc_from_words(k_lo + (((ks >> 2) * (64 * 128) + (ks & 3) * 32) >> 4), kDescHiSw128);
+              const uint32_t add = ks > 0 || term < TERMS - 1 ? 1u : 0u;
+              if (Q_HALF && ks >= 4) umma_bf16(tmem_base + S_COL + q * kKeysPerTile, desc_from_words(p_lo0 + ((q * P_BYTES + (ks & 3) * 32) >> 4), kDescHiSw128), k_desc, idesc_qk, add);
+              else umma_bf16_a_tmem(tmem_base + S_COL + q * kKeysPerTile, tmem_base + Q_COL + q * Q_COLS + term * (DH / 2) + ks * 8, k_desc, idesc_qk, add);
             }
           }
           umma_commit(s_full + q);
@@ -408,7 +423,7 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
       };
       const auto pv = [&](int q, int i) {
         const uint32_t v_lo = v_lo0 + (i % STAGES) * (STAGE_BYTES >> 4);
-        const int pb = 2 * q + (n_pv[q] & 1);
+        const int pb = 2 * q + n_pv[q] % P_BUFS;
         const uint32_t p_lo = p_lo0 + pb * (TERMS * P_BYTES >> 4);
         const uint32_t keep = n_pv[q] > 0 ? 1u : 0u;
         if (elect_one()) {
@@ -418,7 +433,7 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
             for (int kk = 0; kk < kKeysPerTile / 16; ++kk) {
               const uint64_t v_desc = desc_from_words(v_lo + ((kk * 16 * 128) >> 4), kDescHiSw128);
               const uint32_t add = kk > 0 || term < TERMS - 1 ? 1u : keep;
-              if constexpr (P_TMEM) umma_bf16_a_tmem(tmem_base + O_COL + q * DH, tmem_base + P_COL + (pb * TERMS + term) * 32 + kk * 8, v_desc, idesc_pv, add);
+              if constexpr (P_TMEM) umma_bf16_a_tmem(tmem_base + O_COL + q * DH, tmem_base + P_COL + ((q * P_BUFS + n_pv[q] % P_BUFS) * TERMS + term) * 32 + kk * 8, v_desc, idesc_pv, add);
               else umma_bf16(tmem_base + O_COL + q * DH, desc_from_words(p_lo + ((term * P_BYTES + kk * 32) >> 4), kDescHiSw128), v_desc, idesc_pv, add);
             }
           }
@@ -432,7 +447,7 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
       // run while the other's softmax does: 8,192 tokens of 32 heads over 8 of 128 545 us, 649 with one wait for both row tiles' scores and one for
       // their weights. A wait costs this one thread a couple of hundred cycles even when the barrier has long flipped, so a row tile's are
       // one (two: 606 us); but where a few stages are filled by warps, P V and the stage's release come first (KV4, 4 portions of 512 at 2,048
-      // keys: heads of 128 98 us against 107, of 256 210 against 271; not of 192, 163 against 159).
+      // keys: heads of 128 88 us against 96, of 256 210 against 271; not of 192, 163 against 159).
       constexpr bool TOGETHER = !KV4 || (DH == 64 && RT == 2) || DH == 192;
       const BarrierPhase none{nullptr, 0u, false};
       const auto wait = [&](const BarrierPhase& w0, const BarrierPhase& w1, const BarrierPhase& w2) {
@@ -446,7 +461,7 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
           const bool next = on(q, i + 1), last_one = on(q, i - 1);
           const BarrierPhase keys{kv_full + (i + 1) % STAGES, static_cast<uint32_t>(((i + 1) / STAGES) & 1), q == 0 && i + 1 < n_tiles};
           const BarrierPhase taken{s_empty + q, static_cast<uint32_t>((n_qk[q] & 1) ^ 1), next};
-          const BarrierPhase weights{p_full + 2 * q + (n_pv[q] & 1), static_cast<uint32_t>((n_pv[q] >> 1) & 1), last_one};
+          const BarrierPhase weights{p_full + 2 * q + n_pv[q] % P_BUFS, static_cast<uint32_t>(n_pv[q] / P_BUFS & 1), last_one};
           const BarrierPhase values{kv_full + STAGES + (i + STAGES - 1) % STAGES, static_cast<uint32_t>(((i - 1) / STAGES) & 1), RINGS == 2 && q == 0 && i >= 1};
           if (TOGETHER) wait(keys, taken, weights);
           else wait(weights, values, none);
@@ -534,7 +549,7 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
         }
         if (n > 0) {
           // O may be touched once P V of the tile before has retired
-          ok = __all_sync(0xffffffffu, mbar_wait(p_empty + 2 * q + ((n - 1) & 1), ((n - 1) >> 1) & 1, abort_flag, a.status, 13) ? 1 : 0) != 0;
+          ok = __all_sync(0xffffffffu, mbar_wait(p_empty + 2 * q + (n - 1) % P_BUFS, (n - 1) / P_BUFS & 1, abort_flag, a.status, 13) ? 1 : 0) != 0;
           if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
@@ -551,12 +566,12 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
       }
       const float base = m_used == -INFINITY ? 0.0f : m_used;
       float sum4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      // this buffer held P of the tile before the last one: its P V has to have retired
-      const int pb = 2 * q + (n & 1);
+      // this buffer held P of the tile before the last one (of the last one where there is one buffer): its P V has to have retired
+      const int pb = 2 * q + n % P_BUFS;
       uint8_t* p_row = p_rows + (n & 1) * TERMS * P_BYTES;
-      const uint32_t p_tmem = tmem_base + lane_base + P_COL + pb * TERMS * 32;
+      const uint32_t p_tmem = tmem_base + lane_base + P_COL + (q * P_BUFS + n % P_BUFS) * TERMS * 32;
       if constexpr (F32) {
-        ok = __all_sync(0xffffffffu, mbar_wait(p_empty + pb, ((n >> 1) & 1) ^ 1, abort_flag, a.status, 13) ? 1 : 0) != 0;
+        ok = __all_sync(0xffffffffu, mbar_wait(p_empty + pb, (n / P_BUFS & 1) ^ 1, abort_flag, a.status, 13) ? 1 : 0) != 0;
         if (!ok) break;
         if constexpr (P_TMEM) asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
@@ -591,7 +606,7 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
         }
         sums[0] = add_pair(sums[0], sums[1]);
         sum4[0] = low_of(sums[0]), sum4[1] = high_of(sums[0]);
-        ok = __all_sync(0xffffffffu, mbar_wait(p_empty + pb, ((n >> 1) & 1) ^ 1, abort_flag, a.status, 13) ? 1 : 0) != 0;
+        ok = __all_sync(0xffffffffu, mbar_wait(p_empty + pb, (n / P_BUFS & 1) ^ 1, abort_flag, a.status, 13) ? 1 : 0) != 0;
         if (!ok) break;
         if constexpr (P_TMEM) {
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -614,7 +629,7 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
       if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(p_full + pb)) : "memory");
     }
     if (ok && my_tiles > 0) {
-      ok = __all_sync(0xffffffffu, mbar_wait(p_empty + 2 * q + ((my_tiles - 1) & 1), ((my_tiles - 1) >> 1) & 1, abort_flag, a.status, 13) ? 1 : 0) != 0;
+      ok = __all_sync(0xffffffffu, mbar_wait(p_empty + 2 * q + (my_tiles - 1) % P_BUFS, (my_tiles - 1) / P_BUFS & 1, abort_flag, a.status, 13) ? 1 : 0) != 0;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     }
     const bool mine = ok && my_tiles > 0;
