@@ -228,8 +228,8 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
   // columns: the row tiles' scores, their Q (two elements a column, a term behind the other), their accumulators; of one row tile the
   // accumulator first
   constexpr int S_COL = RT == 1 ? DH : 0, Q_COL = S_COL + 64 * RT, O_COL = RT == 1 ? 0 : Q_COL + RT * Form::Q_COLS;
-  constexpr int P_COL = RT * (64 + Form::Q_COLS + DH), P_BUFS = Form::P_BUFS, Q_COLS = Form::Q_COLS;
-  constexpr bool Q_HALF = Form::Q_HALF;      // P_TMEM: [row tile][buffer][term]
+  constexpr int P_COL = RT * (64 + Form::Q_COLS + DH), P_BUFS = Form::P_BUFS, Q_COLS = Form::Q_COLS;      // P_TMEM: [row tile][buffer][term]
+  constexpr bool Q_HALF = Form::Q_HALF;
   constexpr uint32_t TMEM_COLS = 512;
   static_assert(64 * RT + RT * Form::Q_COLS + RT * DH <= 512, "tensor memory");
   constexpr float kRescaleStep = 8.0f;
