@@ -1,0 +1,66 @@
+"""Attention over a cache in 4 bits where there is little to read: sequences and rows without keys, tables that are no wider than they have to
+be, portions that bring more tokens than a call takes. Tolerances: test_kv4_gpu.py."""
+import numpy as np
+import pytest
+import torch
+
+from test_kv4_gpu import Batch, cuda
+from tiny_inference_engine_b200 import ops
+from tiny_inference_engine_b200.errors import TieError
+from tiny_inference_engine_b200.ops import gemm_select
+
+pytestmark = pytest.mark.gpu
+
+
+def narrow(b, page, columns=None):
+    """The batch's tables as wide as its longest context needs (or `columns`), with -1 in every entry that holds no page and behind the last row."""
+    n = len(b.contexts)
+    pages = [-(-c // page) for c in b.contexts]
+    width = max(pages) if columns is None else columns
+    room = np.full(n * width + 64, -1, np.int32)
+    rows = room[:n * width].reshape(n, width)
+    old = b.args[2].cpu().numpy()
+    for i, p in enumerate(pages):
+        rows[i, :min(p, width)] = old[i, :min(p, width)]
+    b.room = cuda(room)
+    b.args = (b.args[0], b.args[1], b.room[:n * width].view(n, width))
+    return b
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("window", [0, 37])
+@pytest.mark.parametrize("contexts,heads,kv_heads,head_dim,page", [([17, 0, 30, 0], 8, 2, 128, 16), ([0, 5, 0], 4, 4, 64, 8), ([1, 0], 71, 1, 64, 1), ([0, 200, 0], 32, 2, 192, 64),
+                                                                  ([3000, 0, 40, 0], 6, 1, 256, 16)])
+def test_tokens_of_sequences_without_keys(dtype, window, contexts, heads, kv_heads, head_dim, page):
+    b = narrow(Batch(len(contexts) + head_dim, contexts, [1] * len(contexts), heads, kv_heads, head_dim, page, dtype, window), page)
+    for hint in (max(contexts), 1, 2 ** 31 - 1):
+        b.out.fill_(9.0)
+        got = b.decode(max_context=hint)           # (looks at the status too: no entry that is no page is asked for)
+        b.check(got)
+        assert (got[[i for i, c in enumerate(contexts) if c == 0]] == 0.0).all()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("window", [0, 16])
+@pytest.mark.parametrize("heads,kv_heads,head_dim,page", [(8, 2, 128, 16), (3, 3, 64, 8), (4, 1, 256, 4), (6, 2, 192, 1)])
+def test_short_portions_with_fewer_keys_than_queries(dtype, window, heads, kv_heads, head_dim, page):
+    b = narrow(Batch(head_dim, [20, 0, 5, 33], [40, 9, 21, 33], heads, kv_heads, head_dim, page, dtype, window), page)
+    got = b.prompt()
+    b.check(got, one_term=True)
+    assert (got[:20] == 0.0).all() and (got[40:49] == 0.0).all() and (got[49:65] == 0.0).all()
+
+
+@pytest.mark.parametrize("columns", [0, 2])
+@pytest.mark.parametrize("window", [0, 64])
+def test_tables_that_are_too_short_are_reported_and_not_read_behind(columns, window):
+    b = narrow(Batch(12, [900, 0, 30], [1] * 3, 8, 2, 64, 16, "bfloat16", window), 16, columns)
+    seqs = cuda([0, 1, 2])
+    ops.attention_kv4_decode(b.qt, b.cache, b.out, *b.args, b.heads, b.scale, seqs, 3, 900, b.work, window=window)
+    torch.cuda.synchronize()
+    with pytest.raises(TieError, match="too short"):
+        gemm_select.check_status()
+    got = b.out.float().cpu().numpy().astype(np.float64).reshape(b.want.shape)
+    b.check(got, [1, 2] if columns else [1])
+    # sequences without keys need no columns at all
+    ops.attention_kv4_decode(b.qt, b.cache, b.out, *b.args, b.heads, b.scale, cuda([1]), 1, 900, b.work, window=window)
+    assert (b.answer()[1] == 0.0).all()

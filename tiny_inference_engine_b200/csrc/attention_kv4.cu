@@ -137,12 +137,14 @@ __global__ void __launch_bounds__(kKv4Threads, NG <= 2 && ROWS <= 8 && !F32 ? 4 
 
   const int* table = a.block_tables + static_cast<long long>(seq) * a.max_blocks;
   // The row of the planes (a token slot of this head) that holds this lane's key of this warp's next tile. Keys beyond the context, below a
-  // window or on a page that cannot be have row 0: what is read there is masked.
+  // window or on a page that cannot be have row 0: what is read there is masked. (hi may be below lo: a context of 0, rows ahead of the first
+  // key, a table that is too short; then no key is looked up.)
+  const unsigned int n_keys = static_cast<unsigned int>(max(hi - lo + 1, 0));
   int next_key = (first + warp) * kKv4Tile + lane;
   const auto row_of_next = [&] {
     const int key = next_key;
     next_key += 4 * kKv4Tile;
-    if (static_cast<unsigned int>(key - lo) > static_cast<unsigned int>(hi - lo)) return 0;
+    if (static_cast<unsigned int>(key - lo) >= n_keys) return 0;
     const int idx = a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size;
     const int page = table[idx];
     if (static_cast<unsigned int>(page) >= static_cast<unsigned int>(a.pages)) {
