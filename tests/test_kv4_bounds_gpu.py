@@ -64,3 +64,27 @@ def test_tables_that_are_too_short_are_reported_and_not_read_behind(columns, win
     # sequences without keys need no columns at all
     ops.attention_kv4_decode(b.qt, b.cache, b.out, *b.args, b.heads, b.scale, cuda([1]), 1, 900, b.work, window=window)
     assert (b.answer()[1] == 0.0).all()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("heads,kv_heads", [(2, 2), (6, 2), (8, 2), (7, 1)])
+@pytest.mark.parametrize("most", [1, 3, 5])
+def test_short_portions_of_more_tokens_than_the_call_takes(dtype, heads, kv_heads, most):
+    """The last block of rows ends inside of a token's neighbours: those are not touched. Every count of rows a CTA (4, 8, 16) and of heads a group."""
+    contexts, queries = [30, 300, 50, 7], [8, 40, 2, 7]
+    b = Batch(most + heads, contexts, queries, heads, kv_heads, 64, 16, dtype)
+    got = b.prompt(max_queries=most)
+    taken = np.concatenate([b.start[i] + np.arange(min(q, most)) for i, q in enumerate(queries)])
+    b.check(got, taken, one_term=True)
+    rest = np.setdiff1d(np.arange(sum(queries)), taken)
+    assert len(rest) and (got[rest] == 9.0).all()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("heads,kv_heads", [(2, 2), (6, 2), (16, 2)])
+def test_tokens_of_listed_sequences_that_bring_several(dtype, heads, kv_heads):
+    """A listed sequence's first row, wherever it sits, and no other."""
+    b = Batch(heads, [40, 2000, 3], [3, 9, 1], heads, kv_heads, 128, 16, dtype)
+    got = b.decode(seqs=[1, 2, 0])
+    b.check(got, [0, 3, 12])
+    assert (np.delete(got, [0, 3, 12], 0) == 9.0).all()

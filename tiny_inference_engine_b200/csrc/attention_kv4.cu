@@ -51,7 +51,7 @@ struct Kv4Args {
   int* counters;            // [grid z][grid x], zero between launches
   int* status;
   long long q_stride, tokens;
-  int max_blocks, pages, q_heads, kv_heads, head_dim, page_size, page_shift, window, max_splits, seqs, row_blocks, min_tiles, q_aligned;
+  int max_blocks, pages, q_heads, kv_heads, head_dim, page_size, page_shift, window, max_splits, seqs, row_blocks, min_tiles, q_aligned, max_queries;
   float scale_log2;
 };
 
@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(kKv4Threads, NG <= 2 && ROWS <= 8 && !F32 ? 4 
   if (seq < 0 || seq >= a.seqs) return;
   const int G = a.q_heads / a.kv_heads;
   const int t0 = a.query_start[seq], nq = a.query_start[seq + 1] - t0, context = a.context_lens[seq];
-  const int rows = min(nq * G - rb * ROWS, ROWS);
+  const int rows = min(min(nq, a.max_queries) * G - rb * ROWS, ROWS);      // (the first max_queries tokens only; the others' rows stay)
   if (rows <= 0 || t0 < 0) return;
   const int pos0 = context - nq;                                           // position of the sequence's first row
   const int q_first = rb * ROWS / G, q_last = (rb * ROWS + rows - 1) / G;
@@ -622,7 +622,7 @@ TIE_API int tie_attention_kv4(int dtype, const void* q, long long q_stride, long
   const Kv4Args a{q, out, static_cast<const uint8_t*>(k_codes), static_cast<const uint8_t*>(v_codes), static_cast<const uint8_t*>(k_words),
                   static_cast<const uint8_t*>(v_words), query_start, context_lens, block_tables, seq_list, scratch, counters, status_word(), q_stride, tokens,
                   max_blocks, static_cast<int>(pages), q_heads, kv_heads, head_dim, page_size, shift, window, static_cast<int>(splits), seqs,
-                  static_cast<int>(row_blocks), min_tiles, q_aligned, scale * 1.4426950408889634f * kKv4Unscale};
+                  static_cast<int>(row_blocks), min_tiles, q_aligned, max_queries, scale * 1.4426950408889634f * kKv4Unscale};
   int st;
   switch (ng) {
     case 1: st = launch_attn_kv4<1>(a, cta_rows, f32, n_list, s); break;
