@@ -160,9 +160,13 @@ class CacheManager:
             import torch
             for g, n in zip(self.groups, self.group_pages):
                 if kv_bits:          # codes and words of every plane's keys and values (zeros stand for zeros)
-                    shape = (len(g.entries), 2, n, g.kv_heads, page_size)
-                    self.storage.append((torch.zeros((*shape, _kv4_row_bytes(g.head_dim) // 9 * 8), dtype=torch.uint8, device=device),
-                                         torch.zeros((*shape, _kv4_row_bytes(g.head_dim) // 18), dtype=torch.int16, device=device)))
+                    shape, width = (n, g.kv_heads, page_size), _kv4_row_bytes(g.head_dim)
+                    # The operators want planes that start on 16 bytes. Codes are 32 bytes a row and more; words may be 4, so a plane of theirs is
+                    # rounded up where its rows make no whole 16 bytes.
+                    words = n * g.kv_heads * page_size * (width // 18)
+                    room = torch.zeros((len(g.entries), 2, -(-words // 8) * 8), dtype=torch.int16, device=device)
+                    self.storage.append((torch.zeros((len(g.entries), 2, *shape, width // 9 * 8), dtype=torch.uint8, device=device),
+                                         room[..., :words].unflatten(-1, (*shape, width // 18))))
                 elif g.value_dim == VALUES_IN_KEYS:
                     self.storage.append(torch.zeros((len(g.entries), 1, n, g.kv_heads, page_size, g.head_dim),
                                                     dtype=dtype, device=device))
