@@ -233,9 +233,10 @@ __global__ void __launch_bounds__(kKv4Threads, NG <= 2 && ROWS <= 8 && !F32 ? 4 
   const int all_to = pos0 + q_first;
 
   const uint32_t signs = kv4_signs();
-  // One tile. EDGE: not every row sees every key of it (its own form, so that the others do without the comparisons)
-  const auto work = [&](auto edge, const uint8_t* stage, int key0) {
-    constexpr bool EDGE = decltype(edge)::value;
+  // One tile. EDGE: not every row sees every key of it (its own form, so that the others do without the comparisons); BIG: with steps that need
+  // a product more (kv4.cuh), in the edges' form whatever the rows see
+  const auto work = [&](auto edge, auto big, const uint8_t* stage, int key0) {
+    constexpr bool EDGE = decltype(edge)::value, BIG = decltype(big)::value;
     // ---- scores, of both halves of the tile side by side
     float sc[2][HN][4];
     uint32_t w[2][2][2 * NG];
@@ -249,8 +250,8 @@ __global__ void __launch_bounds__(kKv4Threads, NG <= 2 && ROWS <= 8 && !F32 ? 4 
         const int key = 16 * b + 8 * h + kappa;
         lds_words(w[b][h], stage + key * CODE_ROW + t * 8 * NG);
         const uint16_t* words = reinterpret_cast<const uint16_t*>(stage + 2 * CODES + key * WORD_ROW);
-        s0[b][h] = kv4_scale(words[(2 * NG * t) >> 2] * 0x10001u, signs);
-        if constexpr (NG > 2) s1[b][h] = kv4_scale(words[((2 * NG * t) >> 2) + 1] * 0x10001u, signs);
+        s0[b][h] = kv4_scale<BIG>(words[(2 * NG * t) >> 2] * 0x10001u, signs);
+        if constexpr (NG > 2) s1[b][h] = kv4_scale<BIG>(words[((2 * NG * t) >> 2) + 1] * 0x10001u, signs);
         else s1[b][h] = s0[b][h];
       }
     }
@@ -265,10 +266,10 @@ __global__ void __launch_bounds__(kKv4Threads, NG <= 2 && ROWS <= 8 && !F32 ? 4 
           const bool second = NG == 4 ? x >= 4 : (NG == 3 ? x >= ((t & 1) ? 2 : 4) : false);
           const Kv4Scale& s = second ? s1[b][h] : s0[b][h];
           const uint32_t word = w[b][h][x], next = word >> 8;
-          v[b][h][0] = kv4_low(word, s);
-          v[b][h][1] = kv4_high(word, s);
-          v[b][h][2] = kv4_low(next, s);
-          v[b][h][3] = kv4_high(next, s);
+          v[b][h][0] = kv4_low<BIG>(word, s);
+          v[b][h][1] = kv4_high<BIG>(word, s);
+          v[b][h][2] = kv4_low<BIG>(next, s);
+          v[b][h][3] = kv4_high<BIG>(next, s);
         }
       }
 #pragma unroll
@@ -334,12 +335,12 @@ __global__ void __launch_bounds__(kKv4Threads, NG <= 2 && ROWS <= 8 && !F32 ? 4 
     uint32_t pf[2][HN][PT][2];
 #pragma unroll
     for (int n = 0; n < HN; ++n) {
-      const float base0 = m[n][0] == -INFINITY ? 0.0f : m[n][0], base1 = m[n][1] == -INFINITY ? 0.0f : m[n][1];
+      const float base0 = m[n][0] == -INFINITY ? 0.0f : kKv4WeightShift - m[n][0], base1 = m[n][1] == -INFINITY ? 0.0f : kKv4WeightShift - m[n][1];
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float p0 = ex2(fmaf(sc[b][n][2 * h], a.scale_log2, -base0)), p1 = ex2(fmaf(sc[b][n][2 * h + 1], a.scale_log2, -base1));
+          const float p0 = ex2(fmaf(sc[b][n][2 * h], a.scale_log2, base0)), p1 = ex2(fmaf(sc[b][n][2 * h + 1], a.scale_log2, base1));
           l[n][0] += p0, l[n][1] += p1;
           uint32_t terms[TWICE ? 2 : PT];
           split_terms<TWICE ? 2 : PT>(p0, p1, terms);
@@ -373,8 +374,8 @@ __global__ void __launch_bounds__(kKv4Threads, NG <= 2 && ROWS <= 8 && !F32 ? 4 
           words[h][0] &= keep, words[h][1] &= keep;
         }
       }
-      const Kv4Scale g0[2] = {kv4_scale(words[0][0], signs), kv4_scale(words[1][0], signs)};
-      const Kv4Scale g1[2] = {SECOND ? kv4_scale(words[0][1], signs) : g0[0], SECOND ? kv4_scale(words[1][1], signs) : g0[1]};
+      const Kv4Scale g0[2] = {kv4_scale<BIG>(words[0][0], signs), kv4_scale<BIG>(words[1][0], signs)};
+      const Kv4Scale g1[2] = {SECOND ? kv4_scale<BIG>(words[0][1], signs) : g0[0], SECOND ? kv4_scale<BIG>(words[1][1], signs) : g0[1]};
 #pragma unroll
       for (int x = 0; x < NG; ++x) {
         const bool second = NG == 3 && ((g * NG) & 3) + x >= 4;
@@ -385,8 +386,8 @@ __global__ void __launch_bounds__(kKv4Threads, NG <= 2 && ROWS <= 8 && !F32 ? 4 
 #pragma unroll
           for (int j = 0; j < 4; ++j) {        // byte j of both keys' words
             const uint32_t both = __byte_perm(vw[2 * h][x], vw[2 * h + 1][x], 0x4400 + 0x1111 * j);
-            v[h][2 * j] = kv4_low(both, s);
-            v[h][2 * j + 1] = kv4_high(both, s);
+            v[h][2 * j] = kv4_low<BIG>(both, s);
+            v[h][2 * j + 1] = kv4_high<BIG>(both, s);
           }
         }
         // (a row's terms one round after the other, so that no product waits for the one ahead of it)
@@ -418,8 +419,17 @@ __global__ void __launch_bounds__(kKv4Threads, NG <= 2 && ROWS <= 8 && !F32 ? 4 
     }
     cp_async_wait<kKv4Stages - 1>();
     __syncwarp();
-    if (key0 < all_from || key0 + kKv4Tile - 1 > all_to) work(std::true_type{}, stage, key0);
-    else work(std::false_type{}, stage, key0);
+    uint32_t big = 0;                     // of this lane's key and value (a key that no row sees: of row 0)
+    {
+      uint32_t words[2][NG];
+      lds_words(words[0], stage + 2 * CODES + lane * WORD_ROW);
+      lds_words(words[1], stage + 2 * CODES + WORDS + lane * WORD_ROW);
+#pragma unroll
+      for (int j = 0; j < NG; ++j) big |= kv4_big(words[0][j]) | kv4_big(words[1][j]);
+    }
+    if (__any_sync(0xffffffffu, (big & kKv4BigBits) != 0)) work(std::true_type{}, std::true_type{}, stage, key0);
+    else if (key0 < all_from || key0 + kKv4Tile - 1 > all_to) work(std::true_type{}, std::false_type{}, stage, key0);
+    else work(std::false_type{}, std::false_type{}, stage, key0);
     __syncwarp();        // (the next fetch writes the stage that was just read)
     if (++at == kKv4Stages) at = 0;
   }

@@ -35,7 +35,9 @@
 // stand there as three bfloat16 terms (24 bits), as the weights do in shared memory. 4 portions of 512 queries at 2,048 keys, 32 heads over 8,
 // us against the kernel whose warps take 16 rows each: heads of 128 88 and 396 (float 195 and 646), of 64 77 and 267 (149 and 407), of 192
 // 148 and 589, of 256 189 and 790. Eight dimensions lie in a tile in the order 0 4 1 5 2 6 3 7, in which a word of codes comes apart; Q is put into tensor
-// memory in the same order and the outputs are taken out of it again. Keys and values are exact in bfloat16, times 2^-64 (kv4.cuh).
+// memory in the same order and the outputs are taken out of it again. Keys and values are exact in bfloat16, times 2^-31 (kv4.cuh).
+#include <type_traits>
+
 #include "attention_mma.cuh"
 #include "kv4.cuh"
 #include "umma.cuh"
@@ -155,15 +157,16 @@ __device__ __forceinline__ void kv4_produce(const UmmaPromptArgs& a, uint8_t* ri
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  const auto put = [&](uint8_t* plane, int row, const uint4& codes, uint32_t words) {
-    const Kv4Scale s = kv4_scale(__byte_perm(words, 0, (group & 1) ? 0x3232 : 0x1010), signs);
+  const auto put = [&](auto big, uint8_t* plane, int row, const uint4& codes, uint32_t words) {
+    constexpr bool BIG = decltype(big)::value;
+    const Kv4Scale s = kv4_scale<BIG>(__byte_perm(words, 0, (group & 1) ? 0x3232 : 0x1010), signs);
     const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
     uint8_t* dst = plane + (group >> 1) * (64 * 128) + row * 128;
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       const uint32_t next = w[c] >> 8;
       *reinterpret_cast<uint4*>(dst + ((((group & 1) * 4 + c) ^ (row & 7)) << 4)) =
-          make_uint4(kv4_low(w[c], s), kv4_high(w[c], s), kv4_low(next, s), kv4_high(next, s));
+          make_uint4(kv4_low<BIG>(w[c], s), kv4_high<BIG>(w[c], s), kv4_low<BIG>(next, s), kv4_high<BIG>(next, s));
     }
   };
   const auto filled = [&](uint64_t* bar) {
@@ -177,43 +180,55 @@ __device__ __forceinline__ void kv4_produce(const UmmaPromptArgs& a, uint8_t* ri
     copy(i);
     find(i + 1);
   }
+  // Tiles from i on; true where the usual form met steps that need a product more (kv4.cuh), and from there on all tiles are taken apart that way. (So
+  // the usual form stays one run of instructions: 4 portions of 512 queries at 2,048 keys, 32 heads over 8 of 128, 90.7 us; with a branch a tile 94, a branch a
+  // word 102, without looking 89.)
+  int i = 0;
+  const auto walk = [&](auto form) {
+    constexpr bool BIG = decltype(form)::value;
 #pragma unroll 1
-  for (int i = 0; i < n_tiles; ++i) {
-    const int st = i % STAGES;
-    asm volatile("cp.async.wait_group %0;" ::"n"(Form::AHEAD - 1) : "memory");
-    const uint8_t* src = raw + (i % Form::AHEAD) * RAW;
-    uint4 kc[PER], vc[PER];
-    uint2 words[PER];
+    for (; i < n_tiles; ++i) {
+      const int st = i % STAGES;
+      asm volatile("cp.async.wait_group %0;" ::"n"(Form::AHEAD - 1) : "memory");
+      const uint8_t* src = raw + (i % Form::AHEAD) * RAW;
+      uint4 kc[PER], vc[PER];
+      uint2 words[PER];
+      uint32_t found = 0;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const int key = (kt_first + i) * kKeysPerTile + first + j * STEP;
-      if (first + j * STEP >= kKeysPerTile) break;
-      kc[j] = *reinterpret_cast<const uint4*>(src + (j * Form::PRODUCERS + id) * 16);
-      vc[j] = *reinterpret_cast<const uint4*>(src + ((PER + j) * Form::PRODUCERS + id) * 16);
-      words[j] = *reinterpret_cast<const uint2*>(src + PER * Form::PRODUCERS * 32 + (j * Form::PRODUCERS + id) * 8);
-      if (key < lo || key > hi) words[j] = make_uint2(0u, 0u);       // what no row sees: zeros
-    }
-    copy(i + Form::AHEAD);          // (this thread's own place, whose words it holds)
-    find(i + Form::AHEAD + 1);
-    uint8_t* k_plane = ring + st * 2 * PLANE_BYTES;
-    if (!__all_sync(0xffffffffu, mbar_wait(kv_empty + st, ((i / STAGES) & 1) ^ 1, abort_flag, a.status, 11) ? 1 : 0)) break;
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      if (first + j * STEP >= kKeysPerTile) break;
-      put(k_plane, first + j * STEP, kc[j], words[j].x);
-      if (Form::RINGS == 1) put(k_plane + PLANE_BYTES, first + j * STEP, vc[j], words[j].y);
-    }
-    if constexpr (Form::RINGS == 2) {
-      filled(kv_full + st);
-      if (!__all_sync(0xffffffffu, mbar_wait(kv_empty + STAGES + st, ((i / STAGES) & 1) ^ 1, abort_flag, a.status, 11) ? 1 : 0)) break;
+      for (int j = 0; j < PER; ++j) {
+        const int key = (kt_first + i) * kKeysPerTile + first + j * STEP;
+        if (first + j * STEP >= kKeysPerTile) break;
+        kc[j] = *reinterpret_cast<const uint4*>(src + (j * Form::PRODUCERS + id) * 16);
+        vc[j] = *reinterpret_cast<const uint4*>(src + ((PER + j) * Form::PRODUCERS + id) * 16);
+        words[j] = *reinterpret_cast<const uint2*>(src + PER * Form::PRODUCERS * 32 + (j * Form::PRODUCERS + id) * 8);
+        if (key < lo || key > hi) words[j] = make_uint2(0u, 0u);       // what no row sees: zeros
+        found |= kv4_big(words[j].x) | kv4_big(words[j].y);
+      }
+      if (!BIG && __any_sync(0xffffffffu, (found & kKv4BigBits) != 0)) return true;
+      copy(i + Form::AHEAD);          // (this thread's own place, whose words it holds)
+      find(i + Form::AHEAD + 1);
+      uint8_t* k_plane = ring + st * 2 * PLANE_BYTES;
+      if (!__all_sync(0xffffffffu, mbar_wait(kv_empty + st, ((i / STAGES) & 1) ^ 1, abort_flag, a.status, 11) ? 1 : 0)) return false;
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
         if (first + j * STEP >= kKeysPerTile) break;
-        put(k_plane + PLANE_BYTES, first + j * STEP, vc[j], words[j].y);
+        put(form, k_plane, first + j * STEP, kc[j], words[j].x);
+        if (Form::RINGS == 1) put(form, k_plane + PLANE_BYTES, first + j * STEP, vc[j], words[j].y);
       }
+      if constexpr (Form::RINGS == 2) {
+        filled(kv_full + st);
+        if (!__all_sync(0xffffffffu, mbar_wait(kv_empty + STAGES + st, ((i / STAGES) & 1) ^ 1, abort_flag, a.status, 11) ? 1 : 0)) return false;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+          if (first + j * STEP >= kKeysPerTile) break;
+          put(form, k_plane + PLANE_BYTES, first + j * STEP, vc[j], words[j].y);
+        }
+      }
+      filled(kv_full + (Form::RINGS - 1) * STAGES + st);
     }
-    filled(kv_full + (Form::RINGS - 1) * STAGES + st);
-  }
+    return false;
+  };
+  if (walk(std::false_type{})) walk(std::true_type{});
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
@@ -564,7 +579,7 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
           asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         }
       }
-      const float base = m_used == -INFINITY ? 0.0f : m_used;
+      const float base = m_used == -INFINITY ? 0.0f : KV4 ? m_used - kKv4WeightShift : m_used;
       float sum4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
       // this buffer held P of the tile before the last one (of the last one where there is one buffer): its P V has to have retired
       const int pb = 2 * q + n % P_BUFS;

@@ -37,14 +37,23 @@ __device__ __forceinline__ uint32_t bf16x2_fma(uint32_t a, uint32_t b, uint32_t 
 }
 // Taking codes apart without shifts. A bfloat16 pattern whose exponent field is 0 or 1 is its lower eight bits as a whole number times 2^-133:
 // subnormal numbers and the first normal ones lie on one line. So a code in bits 0..3 or 4..7 of a half word is a number as it stands, once
-// the other bits are masked away, code 2^-133 or code 2^-129, and one fma with s 2^69 or s 2^65 and -z s 2^-64 makes the value times 2^-64
-// of it, exactly (the products take 2^64 back in float). Against the code put into the mantissa of 16, which takes a shift and two
-// constants: eight contexts of 32,768 keys 81 us against 94 (then); logical operations and shifts share the pipe that bounds these kernels.
-// Scales from 2^57 up count as 2^57, so that s 2^69 stays finite (and NaN stays NaN); values below 2^-62 lose bits.
-constexpr float kKv4Unscale = 18446744073709551616.0f;     // 2^64
+// the other bits are masked away, code 2^-133 or code 2^-129, and one fma with s 2^102 or s 2^98 and -z s 2^-31 makes the value times 2^-31
+// of it, exactly (the products take 2^31 back in float): the least step, 2^-100, leaves whole multiples of 2^-133. Against the code put into the
+// mantissa of 16, which takes a shift and two constants: eight contexts of 32,768 keys 81 us against 94 (then); logical operations and shifts
+// share the pipe that bounds these kernels.
+// s 2^102 is finite for steps below 2^26. Where there are larger ones (BIG), one product more brings the codes to code 2^-6, and s 2^-25 takes them
+// to the same numbers. Whoever takes words apart looks for them first (kv4_big): no model's keys come near, so that costs a few instructions
+// a tile, and attention sees every step of the format.
+constexpr float kKv4Unscale = 2147483648.0f;               // 2^31
+// Weights are 2^8 times what they are (their sums too, so quotients stay): products with the smallest values of the format, 2^-131, then are
+// no subnormal floats, and sums of 2^20 of the largest, 2^120 with weights of up to 2^8, stay below 2^128.
+constexpr float kKv4WeightShift = 8.0f;
+// Two words side by side: whether either's step is 2^26 or above, or NaN: 0x4c80 in bfloat16. (Bits 15 and 31 of the sum, no carry.)
+__device__ __forceinline__ uint32_t kv4_big(uint32_t words) { return words + 0x33803380u; }
+constexpr uint32_t kKv4BigBits = 0x80008000u;
 // `words`: two groups' words, one in each half (the same one twice where both numbers of a pair belong to one group).
 struct Kv4Scale {
-  uint32_t low, high, off;      // for codes in bits 0..3 and 4..7; -z s 2^-64
+  uint32_t low, high, off;      // for codes in bits 0..3 and 4..7; -z s 2^-31
 };
 // (signs: two sign bits, in a register: with a constant the compiler makes two operations of the and-or)
 __device__ __forceinline__ uint32_t kv4_signs() {
@@ -52,19 +61,24 @@ __device__ __forceinline__ uint32_t kv4_signs() {
   asm volatile("mov.b32 %0, 0x80008000;" : "=r"(signs));
   return signs;
 }
-__device__ __forceinline__ Kv4Scale kv4_scale(uint32_t words, uint32_t signs) {
+template <bool BIG> __device__ __forceinline__ Kv4Scale kv4_scale(uint32_t words, uint32_t signs) {
   Kv4Scale k;
   uint32_t z;
-  asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(k.low) : "r"(words & 0xffe0ffe0u), "r"(0x5c005c00u));     // 2^57
-  k.low = bf16x2_mul(k.low, 0x62006200u);                                                           // 2^69
-  k.high = bf16x2_mul(k.low, 0x3d803d80u);                                                          // 2^-4
   asm("lop3.b32 %0, %1, 0x000f000f, %2, 0xEA;" : "=r"(z) : "r"(words), "r"(signs));                  // -z 2^-133
-  k.off = bf16x2_mul(z, k.low);
+  k.low = bf16x2_mul(words & 0xffe0ffe0u, BIG ? 0x33003300u : 0x72807280u);                         // 2^-25, 2^102
+  k.high = BIG ? k.low : bf16x2_mul(k.low, 0x3d803d80u);                                            // 2^-4
+  k.off = bf16x2_mul(BIG ? bf16x2_mul(z, 0x7f007f00u) : z, k.low);                                  // 2^127
   return k;
 }
-// The values 2^-64 of the codes in bits 0..3 (4..7) of both halves of w.
-__device__ __forceinline__ uint32_t kv4_low(uint32_t w, const Kv4Scale& k) { return bf16x2_fma(w & 0x000f000fu, k.low, k.off); }
-__device__ __forceinline__ uint32_t kv4_high(uint32_t w, const Kv4Scale& k) { return bf16x2_fma(w & 0x00f000f0u, k.high, k.off); }
+// The values 2^-31 of the codes in bits 0..3 (4..7) of both halves of w.
+template <bool BIG> __device__ __forceinline__ uint32_t kv4_low(uint32_t w, const Kv4Scale& k) {
+  const uint32_t codes = w & 0x000f000fu;
+  return bf16x2_fma(BIG ? bf16x2_mul(codes, 0x7f007f00u) : codes, k.low, k.off);                    // 2^127
+}
+template <bool BIG> __device__ __forceinline__ uint32_t kv4_high(uint32_t w, const Kv4Scale& k) {
+  const uint32_t codes = w & 0x00f000f0u;
+  return bf16x2_fma(BIG ? bf16x2_mul(codes, 0x7d007d00u) : codes, k.high, k.off);                   // 2^123
+}
 
 // Eight dimensions of a row, `dims` of them there (the others are zero); vec: rows are 16-byte aligned.
 template <typename T>

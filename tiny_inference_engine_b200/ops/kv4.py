@@ -10,8 +10,8 @@ lo = min(0, its least) and hi = max(0, its largest):
 so that every value is a bfloat16 number within s of what was appended, and costs 4.5 bits. Codes lie in padded / 2 bytes, dimension d in
 byte d // 2, the even one in the low bits; a group's 16-bit word holds s as bfloat16 (its low five bits are zero) and z in its low four. A token
 and head whose key or value holds a number that is not finite, or one of magnitude 2^120 or more, gets the key words 0x7fc0, zero
-value words and zero codes: rows that see that key are NaN, no other is. Attention reads steps s from 2^57 up as 2^57, so keys and values are
-to stay below 2^57 in magnitude; what they hold below 2^-62 it may lose.
+value words and zero codes: rows that see that key are NaN, no other is. Attention sees the values that `kv4_read` gives, over the whole range of
+steps (from 2^26 on, which no model's keys come near, with a product more a value).
 """
 from __future__ import annotations
 
