@@ -1,4 +1,5 @@
-"""The planes of a cache in 4 bits that the cache manager makes, over pages and page counts of every alignment: what the operators take."""
+"""The planes of a cache in 4 bits that the cache manager makes, over pages and page counts of every alignment: what the operators take.
+And its option of the command line."""
 import itertools
 
 import pytest
@@ -38,3 +39,9 @@ def test_the_operators_reach_their_last_check(page, heads, pages, head_dim):
     for entry in range(2):
         with pytest.raises(InvalidArgument, match="CUDA"):
             ops.kv4_append(x, x, slots, made.layer_cache(entry, True).kv4)
+
+
+def test_the_command_line_names_the_option_and_refuses_other_bits_before_it_reads_a_model(capsys):
+    from tiny_inference_engine_b200.cli.main import main
+    assert main(["--help"]) == 0 and "--kv-bits" in capsys.readouterr().out
+    assert main(["generate", "-m", "x", "-p", "1", "--kv-bits", "8"]) == 1 and "kv_bits must be 4" in capsys.readouterr().err

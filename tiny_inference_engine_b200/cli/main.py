@@ -33,6 +33,7 @@ generate options:
   --max-tokens N        tokens to generate (default 256)
   --kv-mem SIZE         KV cache budget, e.g. 4G or 512M (default 4G)
   --page-size P         tokens per cache page (default 16)
+  --kv-bits 0|4         4: keys and values in 4 bits; 0: in the compute type (default 0)
   --max-seqs S          sequences per step (default 64)
   --max-tokens-per-step B  tokens per step (default 512)
   --policy fcfs|srpt-aging  admission order (default srpt-aging)

@@ -66,6 +66,8 @@ def load_engine(model_dir, dtype="bfloat16", kv_mem: int = 4 << 30, page_size: i
     """Model folder -> Engine, wired the way the reference's CLI wires its own (src/cli/main.cpp:33-69). `kv_bits` as in `make_cache`."""
     serving = serving or ServingConfig()
     serving.validate()
+    if kv_bits not in (0, 4):       # (the cache refuses it too, but only once the weights have been read)
+        raise InvalidArgument(f"kv_bits must be 4, or 0 for the compute type, got {kv_bits}")
     model = load_model(model_dir, dtype, device, random_weights, seed)
     # Requests that hold pages or a state slot at one time: those running, and those whose last token is still
     # on its way from the GPU when the step behind it was already decided (they have left the scheduler).
