@@ -4,10 +4,10 @@ import numpy as np
 import pytest
 import torch
 
-from test_kv4_gpu import Batch, cuda
+from test_kv4_gpu import DT, PROMPT, Batch, cuda
 from tiny_inference_engine_b200 import ops
 from tiny_inference_engine_b200.errors import TieError
-from tiny_inference_engine_b200.ops import gemm_select
+from tiny_inference_engine_b200.ops import gemm_select, kv4
 
 pytestmark = pytest.mark.gpu
 
@@ -88,3 +88,48 @@ def test_tokens_of_listed_sequences_that_bring_several(dtype, heads, kv_heads):
     got = b.decode(seqs=[1, 2, 0])
     b.check(got, [0, 3, 12])
     assert (np.delete(got, [0, 3, 12], 0) == 9.0).all()
+
+
+@pytest.mark.parametrize("window", [0, 29])
+@pytest.mark.parametrize("contexts,queries,heads,kv_heads,head_dim,page", PROMPT)
+def test_short_portions_have_weights_of_two_terms(window, contexts, queries, heads, kv_heads, head_dim, page):
+    """Rows that are not 16-byte aligned stay with the kernel of few rows, whatever their number: weights enter with 16 bits."""
+    b = Batch(len(contexts) * 13 + head_dim, contexts, queries, heads, kv_heads, head_dim, page, "bfloat16", window)
+    assert b.qt.stride(0) % 8
+    b.check(b.prompt(), one_term=False)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_planes_of_more_than_4_gb(monkeypatch, dtype):
+    """A sequence's pages at the far end of the planes give the bits that they give at the near one: append, read, tokens and both kinds of portions."""
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("planes of 10 GB")
+    kv_heads, heads, dim, page, n = 2, 8, 256, 64, 300
+    pages = (1 << 32) // (kv_heads * page * dim // 2) + 8              # a plane of codes: 2^32 bytes and 8 pages more
+    big, small = ops.kv4_cache(pages, kv_heads, page, dim), ops.kv4_cache(5, kv_heads, page, dim)
+    assert big.k_codes.numel() > 1 << 32
+    rng = np.random.default_rng(3)
+    k, v = (cuda(rng.standard_normal((n, kv_heads * dim)), DT[dtype]) for _ in range(2))
+    q = cuda(rng.standard_normal((n, heads * dim)), DT[dtype])
+    work = ops.kv4_workspace(heads, kv_heads, dim)
+    got = []
+    for cache, first in ((small, 0), (big, pages - 5)):
+        table = first + np.array([[3, 1, 0, 4, 2]])
+        at = np.arange(n)
+        slots = cuda(table[0, at // page] * page + at % page)
+        assert int(slots.max()) < 2 ** 31
+        ops.kv4_append(k, v, slots, cache)
+        out = [torch.empty_like(x) for x in (k, v, q, q, q)]
+        ops.kv4_read(cache, slots, out[0], out[1])
+        for i, min_groups, rows in ((2, 1 << 30, n), (3, 0, n), (4, 0, 1)):
+            monkeypatch.setattr(kv4, "UMMA_GROUPS", min_groups), monkeypatch.setattr(kv4, "UMMA_FEW_GROUPS", min_groups)
+            out[i].zero_()
+            args = q, cache, out[i], cuda([0, rows]), cuda([n]), cuda(table)
+            if rows == 1:
+                ops.attention_kv4_decode(*args, heads, dim ** -0.5, cuda([0]), 1, n, work)
+            else:
+                ops.attention_kv4_prompt(*args, 1, n, heads, dim ** -0.5, n, work)
+        torch.cuda.synchronize()
+        gemm_select.check_status()
+        got.append(out)
+    assert all(torch.equal(x, y) for x, y in zip(*got)) and bool((got[0][3] != 0).any(1).all())
