@@ -23,8 +23,9 @@
 // instructions than a tile's cp.asyncs and their addresses.) At the end the warps put their sums together in shared memory, and the
 // splits theirs in the workspace: the last CTA to arrive adds them in split order, so the result does not depend on who came last.
 // Measured (one B200, in a graph): 32 heads over 8 of 128, eight contexts of 32,768 keys 74 us: 302 MB at 4.1 TB/s, 0.63 of the copy rate; 64 contexts of 512
-// to 4,096 keys 52 us; one of 4,096 keys 9.7 us. Counters of the first: 175 instructions a warp for 8 keys, 2.3 instructions a cycle and
-// SM, logical pipe 50 %, fma pipe 34 %, tensor pipe 21 %: what remains is two-cycle operations that get in one another's way.
+// to 4,096 keys 52 us; one of 4,096 keys 9.6 us. Counters of the first with half the keys: 178 instructions a warp for 8 keys, 2.3 a cycle and
+// SM of 4, logical pipe 49 %, fma pipe 33 %, tensor pipe 20 %, 16 warps an SM: no unit is full. What bounds it is the work of a key, and warps too few
+// (for their registers) to hide what waits for other work or for a pipe that is taken.
 //
 // The weights enter the second product as two bfloat16 terms (16 bits), the queries of float rows and their weights as three (24 bits):
 // the operands then have the bits that the result's type can show.

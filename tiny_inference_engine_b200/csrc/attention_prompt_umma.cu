@@ -33,8 +33,8 @@
 // Warps take the place of the TMA producer: they read codes and words some tiles ahead, take them apart and write the
 // tile as TMA would have. Heads above 128 leave tensor memory for one row tile a CTA; so do float queries, which
 // stand there as three bfloat16 terms (24 bits), as the weights do in shared memory. 4 portions of 512 queries at 2,048 keys, 32 heads over 8,
-// us against the kernel whose warps take 16 rows each: heads of 128 88 and 396 (float 195 and 646), of 64 77 and 267 (149 and 407), of 192
-// 148 and 589, of 256 189 and 790. Eight dimensions lie in a tile in the order 0 4 1 5 2 6 3 7, in which a word of codes comes apart; Q is put into tensor
+// us against the kernel whose warps take 16 rows each: heads of 128 90 and 405 (float 194 and 655), of 64 79 and 280 (148 and 422), of 192
+// 148 and 604, of 256 193 and 803. Eight dimensions lie in a tile in the order 0 4 1 5 2 6 3 7, in which a word of codes comes apart; Q is put into tensor
 // memory in the same order and the outputs are taken out of it again. Keys and values are exact in bfloat16, times 2^-31 (kv4.cuh).
 #include <type_traits>
 
@@ -459,7 +459,7 @@ attn_prompt_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
       };
       // Step i, for row tile 0 and then for row tile 1: P V of key tile i - 1, once the softmax has written its weights, and Q K^T of key tile
       // i + 1, once it has taken the scores of tile i, which happens right behind that. The row tiles have waits of their own, so one's products
-      // run while the other's softmax does: 8,192 tokens of 32 heads over 8 of 128 545 us, 649 with one wait for both row tiles' scores and one for
+      // run while the other's softmax does: 8,192 tokens of 32 heads over 8 of 128 545 us (517 now), 649 with one wait for both row tiles' scores and one for
       // their weights. A wait costs this one thread a couple of hundred cycles even when the barrier has long flipped, so a row tile's are
       // one (two: 606 us); but where a few stages are filled by warps, P V and the stage's release come first (KV4, 4 portions of 512 at 2,048
       // keys: heads of 128 88 us against 96, of 256 210 against 271; not of 192, 163 against 159).
@@ -798,10 +798,10 @@ static void cut_prompt_umma(UmmaPromptArgs& a, int max_queries, int n_seqs, int 
   int sms = 148;
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, 0);
   // ...; with many keys they share out the keys instead: what bounds either is the keys and values that L2 feeds the SMs, and tiles of
-  // 256 rows read them half as often. 128 rows a CTA against shares, us (with one wait for both row tiles, up to
-  // a tenth slower than now): two shares, 512 tokens of 32 heads over 8, heads of 128: 2,100 keys 45 / 43, 3,000 57 / 51, 8,192 131 / 100, 16,384 246 / 175 (at 1,024 24 / 29: the merge costs about 8 us); heads of 64 37 / 37,
-  // 47 / 45, 111 / 92, 207 / 164. Four shares, 128 tokens: heads of 128 2,100 keys 43 / 37, 3,000 55 / 41, 8,192 126 / 65; 16 heads of 64 over
-  // 4 35 / 31, 45 / 35, 104 / 57; 8 over 8 of 128 41 / 29, 53 / 31, 124 / 49.
+  // 256 rows read them half as often. 128 rows a CTA against shares, us: two shares, 512 tokens of 32 heads over 8, heads of 128: 2,100 keys
+  // 35.9 / 33.8, 3,000 47.8 / 41.0, 8,192 115 / 81, 16,384 224 / 147 (at 1,024 21.7 / 24.8: the merge costs about 8 us); heads of 64 28.9 / 26.9, 38.1 / 33.3,
+  // 93 / 73, 179 / 135 (17.1 / 18.8). Four shares, 128 tokens: heads of 128 2,100 keys 35.5 / 30.1, 3,000 47.0 / 33.1, 8,192 114 / 53; 16 heads of 64 over
+  // 4 28.3 / 22.0, 37.3 / 25.0, 91 / 45; 8 over 8 of 128 34.4 / 22.1, 46.0 / 24.6, 113 / 42.
   const long long ctas = static_cast<long long>(a.kv_heads) * ceil_div(max_rows, 256) * n_seqs;
   const int keys = a.window > 0 && a.window + max_queries < max_keys ? a.window + max_queries : max_keys;
   if (ctas * 2 <= sms) {
@@ -812,10 +812,12 @@ static void cut_prompt_umma(UmmaPromptArgs& a, int max_queries, int n_seqs, int 
 
 // The same with KV4, by what the ways cost in tiles of 64 keys by 256 rows: the CTAs' rounds on the SMs times a CTA's tiles. Two shares of the
 // keys add the time of 8 tiles to a round, four 12 (and four CTAs of a cluster find room on about 132 of the SMs); CTAs of 128 rows take 0.86 of a
-// tile's time. How many CTAs have rows is estimated from all rows of the step, since portions differ. Against what was measured (us): portions
-// of 512, 342, 172 and 2 tokens of 16 heads of 64 over 4 at 8,192 keys: one share 170, two 96, four 151 (the rule: two); 512 tokens of
-// 32 heads of 128 over 8 at 8,192 keys 184, 107, 135 (two); 128 tokens at 4,096 keys 98, 63, 47 (four); 1,024 tokens at 4,096 keys 100, 115, 176
-// (one); eight portions of 300 to 2 tokens at 4,096 keys 184, 176, 235 (two); 300 tokens at 300 keys 17.7, 22, 42, 128 rows 16.1 (128 rows).
+// tile's time. How many CTAs have rows is estimated from all rows of the step, since portions differ. (The terms were fitted when a tile took a
+// tenth to a third longer; a merge is about 11 tiles now.) What it picks, against all ways, us: portions of 512, 342, 172 and 2 tokens of 16 heads of
+// 64 over 4 at 8,192 keys: one share 146, of 128 rows 137, two shares 83, four 142 (the rule: two); 512 tokens of 32 heads of 128 over 8 at 8,192 keys 158, 144,
+// 93, 123 (two); 128 tokens at 4,096 keys 84, 76, 55, 41 (four); 1,024 tokens at 4,096 keys 86, 134, 102, 163 (one); eight portions of 300 to 2 tokens at
+// 4,096 keys 168, 225, 164, 239 (two); 300 tokens at 300 keys 14.7, 13.0, 19.6, 39 (128 rows); 2,048 tokens at 2,048 keys 55, 94, 105, 218 (one). Forms of one
+// row tile, 512 tokens at 8,192 keys, one, two and four shares: heads of 192 139, 155, 200, of 256 193, 210, 262, float of 128 184, 198, 236 (one).
 static void cut_prompt_kv4(UmmaPromptArgs& a, int row_tiles, int max_queries, int n_seqs, int max_keys) {
   const long long group = a.q_heads / a.kv_heads, max_rows = max_queries * group;
   const int keys = a.window > 0 && a.window + max_queries < max_keys ? a.window + max_queries : max_keys;

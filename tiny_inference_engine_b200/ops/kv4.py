@@ -91,9 +91,9 @@ def _fail(msg: str):
 # When the tcgen05 kernel takes the portions of a prompt, in place of the one whose warps take 16 rows each: from UMMA_MIN_ROWS rows (queries x heads
 # of a group) a portion, and UMMA_GROUPS of 16 rows in all, or with long contexts UMMA_FEW_GROUPS (groups x keys UMMA_GROUPS x 1,024). It starts
 # slower (9 to 15 us a call against 5 to 10) and its tiles of 128 rows are too few for the GPU until then. bfloat16, 32 heads over 8 of 128, us with
-# it and without: 64 portions of 16 rows at 512 keys 69 and 26, 32 of 48 rows at 64 18 and 21, 16 of 64 rows 10 and 15; one of 64 queries at 300 keys (128
-# groups) 18 and 10, 128 at 1,024 (256 groups) 29 and 20, at 2,048 35 and 44, 192 at 1,024 (384 groups) 29 and 33, 512 at 512 20 and 38; 4
-# of 512 at 2,048 97 and 396. float32: 64 at 300 20 and 11, 192 at 1,024 34 and 44, 4 of 512 at 2,048 195 and 646.
+# it and without: 64 portions of 16 rows at 512 keys 62 and 27, 32 of 48 rows at 64 16 and 23, 16 of 64 rows 9 and 16; one of 64 queries at 300 keys (128
+# groups) 15 and 11, 128 at 1,024 (256 groups) 27 and 22, at 2,048 34 and 47, 192 at 1,024 (384 groups) 26 and 36, 512 at 512 17 and 38; 4
+# of 512 at 2,048 91 and 406. float32: 64 at 300 20 and 11, 192 at 1,024 33 and 45, 4 of 512 at 2,048 195 and 656.
 UMMA_MIN_ROWS, UMMA_GROUPS, UMMA_FEW_GROUPS = 48, 384, 128
 _NO_UMMA_ATTENTION = os.environ.get("TIE_NO_UMMA_ATTENTION") == "1"
 _FLOATS = {torch.float32: 0, torch.bfloat16: 1}
