@@ -133,3 +133,61 @@ def test_planes_of_more_than_4_gb(monkeypatch, dtype):
         gemm_select.check_status()
         got.append(out)
     assert all(torch.equal(x, y) for x, y in zip(*got)) and bool((got[0][3] != 0).any(1).all())
+
+
+def test_step_tables_of_the_most_sequences_and_requests_and_of_more():
+    from tiny_inference_engine_b200.errors import InvalidArgument
+    n, held = 8192, 1 << 17
+    state = dict(lens=cuda(np.zeros(held)), tables=cuda(np.zeros((held, 2))), free_pages=cuda(np.arange(2 * n)), free_count=cuda([2 * n]))
+    who = np.random.default_rng(0).permutation(held)[:n]
+    arrays = ops.step_arrays(n, 3 * n, 2)
+    ops.step_tables(cuda(who), cuda(np.full(n, 3)), **state, page_size=2, arrays=arrays)
+    assert int(arrays.status) == 0 and int(arrays.free_left) == 0 and int(state["free_count"]) == 0
+    assert np.array_equal(state["lens"].cpu().numpy()[who], np.full(n, 3)) and int(state["lens"].sum()) == 3 * n
+    # pages come off the end of the stack, in the order of the sequences
+    assert np.array_equal(arrays.block_tables.cpu().numpy().reshape(-1), np.arange(2 * n)[::-1])
+    pages = arrays.block_tables.cpu().numpy()
+    assert np.array_equal(arrays.slots.cpu().numpy().reshape(n, 3), np.stack([pages[:, 0] * 2, pages[:, 0] * 2 + 1, pages[:, 1] * 2], 1))
+    status = cuda([7])
+    ops.release_tables(cuda(who), **state, page_size=2, status=status)
+    assert int(status) == 0 and int(state["free_count"]) == 2 * n and int(state["lens"].abs().sum()) == 0
+    assert np.array_equal(state["free_pages"].cpu().numpy(), np.arange(2 * n)[::-1])
+    with pytest.raises(InvalidArgument, match="8193 sequences"):
+        ops.step_tables(cuda(np.full(n + 1, -1)), cuda(np.zeros(n + 1)), **state, page_size=2, arrays=ops.step_arrays(n + 1, 4, 2))
+    with pytest.raises(InvalidArgument, match="8193 sequences"):
+        ops.release_tables(cuda(np.full(n + 1, -1)), **state, page_size=2, status=status)
+    state["lens"], state["tables"] = cuda(np.zeros(held + 1)), cuda(np.zeros((held + 1, 2)))
+    with pytest.raises(InvalidArgument, match="131073 requests"):
+        ops.step_tables(cuda([0]), cuda([1]), **state, page_size=2, arrays=ops.step_arrays(1, 4, 2))
+
+
+def test_entries_of_a_list_that_name_no_sequence_are_left_out():
+    b = Batch(19, [40, 900], [1, 1], 8, 2, 64, 16, "bfloat16")
+    got = b.decode(seqs=[-1, 1, 2, 2 ** 31 - 1])
+    b.check(got, [1])
+    assert (got[0] == 9.0).all()
+
+
+def test_calls_of_two_graphs_that_run_at_the_same_time():
+    """Each with a workspace of its own, replayed in two streams; and one after the other with one workspace."""
+    a, b = (Batch(50 + i, [4000, 300], [1, 1], 8, 2, 128, 16, "bfloat16") for i in range(2))
+    want = [a.decode(), b.decode()]
+    seqs, graphs = cuda([0, 1]), []
+    for x, work in ((a, a.work), (b, b.work), (b, a.work)):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            x.out.fill_(9.0)
+            ops.attention_kv4_decode(x.qt, x.cache, x.out, *x.args, x.heads, x.scale, seqs, 2, 4000, work)
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    for x, w in zip((a, b), want):
+        assert np.array_equal(x.answer(), w)
+    for _ in range(5):
+        graphs[0].replay(), graphs[2].replay()
+    for x, w in zip((a, b), want):
+        assert np.array_equal(x.answer(), w)

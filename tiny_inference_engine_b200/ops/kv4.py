@@ -324,7 +324,7 @@ def step_tables(requests, counts, lens, tables, free_pages, free_count, page_siz
     they stay (a step that is planned again gets the same pages).
     A step that cannot be is refused whole: arrays.status gets the TABLES_* bits that say why (too few free pages; a request longer than
     `tables` or the block tables are wide; more rows than the arrays have; a request outside of lens, a negative count or length, a request
-    named twice), every slot is -1, every context and query_start 0, and the state stays as it was."""
+    named twice), every slot is -1, every context and query_start 0, and the state stays as it was. At most 8,192 sequences of 131,072 requests."""
     what = "step_tables"
     n, held, width, pages = _check_tables(what, requests, lens, tables, free_pages, free_count, page_size)
     query_start, context_lens, positions, seq_of_row, slots, block_tables, free_left, status = arrays
@@ -347,7 +347,7 @@ def step_tables(requests, counts, lens, tables, free_pages, free_count, page_siz
 def release_tables(requests, lens, tables, free_pages, free_count, page_size: int, status) -> None:
     """The pages of `requests` (int32, no request twice, -1 is skipped) go back onto the end of the stack, the requests in their order and each one's
     pages in theirs, as `CacheManager.release` gives them back; their lengths become 0. Refused whole, with the TABLES_* bits in `status`
-    (int32 [1], else 0), where a request or length cannot be or the stack would overflow."""
+    (int32 [1], else 0), where a request or length cannot be or the stack would overflow. At most 8,192 of 131,072 requests."""
     what = "release_tables"
     n, held, width, pages = _check_tables(what, requests, lens, tables, free_pages, free_count, page_size)
     if status.dtype is not _I32 or status.numel() != 1:
